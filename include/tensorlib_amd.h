@@ -372,6 +372,121 @@ int tl_hgemm_silu_mul_f16(const void* X, const void* W13, void* scratch, void* o
  * (model/llama2_7b/src/Transformer.cpp:231-261). */
 int tl_causal_mask_f16(void* mask, int reps, int seqlen, int start_pos);
 
+/* ------------------------------------ several sequences over a paged key-value cache ---- */
+
+/* The reference decodes one sequence over a contiguous cache (model/llama2_7b/src/Transformer.cpp:47-109) and picks
+ * greedily (model/llama2_7b/src/llama2.cpp:81-91); the entries of this section have no counterpart in it.  They serve a
+ * batch of sequences of different lengths whose caches lie in pages of one pool, and beam search over it.
+ *
+ * A page holds page_size consecutive positions of all kv heads of one layer's keys (or values).  tables[seq][i] is the
+ * page of positions [i * page_size, (i + 1) * page_size) of a sequence, -1 behind its last page; table_stride entries per
+ * sequence.  tables, lens, positions, ids and counts are DEVICE int32 arrays, read when the kernels run, so a captured
+ * graph follows them from replay to replay.  Entries out of range never lead to an access out of bounds; each entry
+ * says what they do instead.  No entry of this section keeps state or scratch in the library: what a call needs beyond
+ * its operands is a workspace of the caller, which calls that may overlap must not share. */
+
+/* One layer's pages.  Element (page p, position row r, kv head h, dim d) lies at p * page_stride + r * row_stride +
+ * h * head_stride + d, in elements, the same for keys and values; strides are multiples of 8, pointers 16-byte aligned,
+ * so both [page][row][head][dim] and [page][head][row][dim] can be described.  head_dim is a multiple of 8 up to 256. */
+typedef struct tl_kv_pages {
+    void* k;
+    void* v;
+    size_t page_stride, row_stride, head_stride;
+    int n_pages, page_size, n_kv_heads, head_dim;
+} tl_kv_pages;
+
+/* Layouts of the pairs that are rotated together: (0,1), (2,3), .. or (i, i + rotary_dim/2). */
+#define TL_ROTARY_INTERLEAVED 0
+#define TL_ROTARY_HALF 1
+/* Frequencies f_i = base^(-2i/rotary_dim), i < rotary_dim/2, in radians per position, and how they are scaled for
+ * contexts longer than the one a model was trained on:
+ *   LINEAR  f_i / factor
+ *   BASE    base replaced by base * factor^(rotary_dim / (rotary_dim - 2)): the last pair slows down by `factor`
+ *   PARTS   with r_i = original_context * f_i / 2 pi turns over the original context: f_i where r_i >= fast_turns,
+ *           f_i / factor where r_i <= slow_turns, linear in r_i between. */
+#define TL_ROTARY_SCALE_NONE 0
+#define TL_ROTARY_SCALE_LINEAR 1
+#define TL_ROTARY_SCALE_BASE 2
+#define TL_ROTARY_SCALE_PARTS 3
+/* Writes rotary_dim/2 doubles to HOST memory.  Needs no GPU. */
+int tl_rotary_frequencies(double* host_out, int rotary_dim, double base, int scaling, double factor, double original_context,
+                          double slow_turns, double fast_turns);
+
+/* out[t,h,:] = in[t,h,:] with its first rotary_dim elements rotated by positions[t] * freq[i] and scaled by `magnitude`;
+ * the rest of the head is copied.  freq: rotary_dim/2 DEVICE doubles.  Angles in fp64, the rotation in fp32, one rounding
+ * (tl_apply_rotary_emb_f16 reproduces the reference's rounding after every operation instead).  Rows of n_heads * head_dim
+ * elements, in_stride / out_stride elements apart; any head_dim, even rotary_dim <= head_dim, any int32 position.
+ * out == in with equal strides is allowed.  16-byte accesses where pointers and strides allow them and rotary_dim is a
+ * multiple of 8 (interleaved) or 16 (half) with head_dim % 8 == 0, else element by element. */
+int tl_rotary_f16(void* out, size_t out_stride, const void* in, size_t in_stride, const int* positions, const double* freq, int rotary_dim,
+                  int layout, float magnitude, int n_tokens, int n_heads, int head_dim);
+
+/* tl_rotary_f16 of q into q_out ([n_tokens, n_heads, head_dim]) and of k into its cache rows, and v copied to its cache
+ * rows, in one launch: token t goes to position positions[t] of sequence seq_ids[t] (NULL: sequence t).  q, k, v rows may
+ * be column blocks of one projection.  A token whose sequence is not in [0, n_seqs), whose position is negative or past
+ * the table, or whose page is not in [0, n_pages) is not stored (its q is still rotated): seq_ids of -1 pad a batch.
+ * Two tokens of one call must not have the same cache row. */
+int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v, size_t v_stride,
+                           const int* positions, const int* seq_ids, const double* freq, int rotary_dim, int layout, float magnitude,
+                           int n_tokens, int n_heads, const tl_kv_pages* cache, const int* tables, size_t table_stride, int n_seqs);
+
+/* Attention of one token per sequence: out[b,h,:] = softmax(scale * q[b,h,:] . K[0:lens[b], g(h), :]^T) . V[0:lens[b], g(h), :]
+ * with g(h) = h / (n_heads / n_kv_heads).  q rows of n_heads * head_dim elements are q_stride apart, out is dense.
+ * lens counts the cached positions, the token's own among them; max_len is the caller's bound on it, which sizes the
+ * launch and the workspace (tl_paged_attention_workspace bytes, 0 if it needs none; nothing in it has to be cleared or
+ * survives the call).  lens[b] <= 0 gives zeros; lens[b] beyond max_len or the table, or a page out of range among the
+ * pages it covers, gives NaN for that sequence.  Scores, weights and sums are fp32, one rounding at the end.
+ * At most 65535 sequences. */
+size_t tl_paged_attention_workspace(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len);
+int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_kv_pages* cache, const int* tables, size_t table_stride,
+                           const int* lens, int n_seqs, int n_heads, int max_len, float scale, void* workspace, size_t workspace_bytes);
+
+/* The pages of a pool are counted in refs[n_pages]: how many table entries name a page, 0 = free.  Entries that a
+ * program counts there for itself (a prompt kept for later) stay counted.  At most 8192 sequences.
+ *
+ * tl_pages_fork: row i of the new state continues sequence parents[i] of the old one; a parent out of [0, n_seqs) leaves
+ * the row empty.  Full pages are shared.  The first row of a parent keeps its partly filled last page, every further
+ * one gets a page of its own: copy_src[i] -> copy_dst[i] (-1, -1 where nothing is to be copied), to be carried out with
+ * tl_pages_copy before the page is read or written.  New pages are the lowest free ones, in row order, pages that this
+ * call frees among them.  *missing = 0, or the number of pages that were lacking: then the new state is the old one and
+ * nothing is to be copied.  The new arrays must not overlap the old ones.
+ * tl_pages_extend: room for add[i] >= 0 more positions of every sequence, in place; lens grows by add.  All or nothing:
+ * *missing = 0, the number of pages that were lacking, or -1 if a table or lens is too short for its sequence.
+ * tl_pages_free: rows[i] != 0 gives sequence i's pages back and empties it, in place.
+ * tl_pages_compact: the live pages move to the low end of the pool.  copy_src / copy_dst ([n_pages]) receive *count moves
+ * (-1 behind them) from pages at or above the number of live pages to free pages below it, both ascending; remap
+ * ([n_pages]) is a live page's new id, -1 for a free one.  tables_out may be tables; refs_out must not overlap refs. */
+int tl_pages_fork(const int* tables, const int* lens, const int* refs, const int* parents, int* tables_out, int* lens_out, int* refs_out,
+                  int* copy_src, int* copy_dst, int* missing, int n_seqs, int table_stride, int n_pages, int page_size);
+int tl_pages_extend(int* tables, int* lens, int* refs, const int* add, int* missing, int n_seqs, int table_stride, int n_pages, int page_size);
+int tl_pages_free(int* tables, int* lens, int* refs, const uint8_t* rows, int n_seqs, int table_stride, int n_pages, int page_size);
+int tl_pages_compact(const int* tables, const int* refs, int* tables_out, int* refs_out, int* remap, int* copy_src, int* copy_dst, int* count,
+                     int n_seqs, int table_stride, int n_pages);
+/* Copies page src[i] to page dst[i] in each of n_planes planes (the keys and the values of every layer), i < *count (device;
+ * NULL: max_pairs), i < max_pairs; pairs with an id out of [0, n_pages) are skipped.  Page p of plane l is the page_bytes
+ * bytes at pool + l * plane_stride + p * page_stride (bytes, multiples of 16).  No page may be a source and a destination,
+ * or a destination twice. */
+int tl_pages_copy(void* pool, size_t plane_stride, size_t page_stride, size_t page_bytes, int n_planes, int n_pages, const int* src, const int* dst,
+                  const int* count, int max_pairs);
+
+/* Beam selection: row r = request * n_beams + beam of logits (fp16, rows logits_stride apart) continues at
+ * scores[r] + log softmax(logits[r])[token]; the best n_select continuations of each request go to scores_out, tokens_out and
+ * parents_out ([n_batch, n_select], the parent as a row r), best first, equal scores by the lower beam, then the lower
+ * token.  finished (bytes, may be NULL): a finished row continues only with end_token, at its own score.  Everything
+ * else is at -inf and follows in the same order: other tokens of a finished row, all tokens of a row whose logits
+ * hold NaN or +inf or nothing but -inf, or whose score is not finite.  Row sums and comparisons in fp64.
+ * n_select <= 64, n_beams <= 1024, at most 65535 rows. */
+size_t tl_beam_select_workspace(int n_batch, int n_beams, int vocab, int n_select);
+int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, const void* logits, size_t logits_stride, const float* scores,
+                       const uint8_t* finished, int n_batch, int n_beams, int vocab, int n_select, int end_token, void* workspace,
+                       size_t workspace_bytes);
+/* The histories ([.., stride] int32, lens valid tokens each) after a selection: row i of the new ones is parents[i]'s, with
+ * tokens[i] appended unless that one is finished; zeros behind.  finished_out: the parent is finished, the token is
+ * end_token, the history is full (the token is then dropped), or the parent is out of [0, n_in) (an empty row).
+ * finished may be NULL.  The new arrays must not overlap the old ones.  At most 65535 rows. */
+int tl_beam_advance(int* history_out, int* lens_out, uint8_t* finished_out, const int* history, const int* lens, const uint8_t* finished,
+                    const int* parents, const int* tokens, int n_in, int n_out, int stride, int end_token);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,16 @@ def declared_symbols() -> list[str]:
 _c = ctypes
 _vp, _sz, _i, _f, _u16 = _c.c_void_p, _c.c_size_t, _c.c_int, _c.c_float, _c.c_uint16
 _ip = _c.POINTER(_c.c_int)
+_d = _c.c_double
+
+
+class KvPages(_c.Structure):
+    """tl_kv_pages: one layer's pages."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _sz), ("row_stride", _sz), ("head_stride", _sz),
+                ("n_pages", _i), ("page_size", _i), ("n_kv_heads", _i), ("head_dim", _i)]
+
+
+_kvp = _c.POINTER(KvPages)
 
 # name -> (restype, argtypes); status-returning functions have restype int
 _PROTOS = {
@@ -107,6 +117,19 @@ _PROTOS = {
     "tl_rope_table_f16": (_i, [_vp, _i, _i]),
     "tl_rope_qk_store_kv_f16": (_i, [_vp, _vp, _vp, _i, _i, _i]),
     "tl_add_rms_norm_f16": (_i, [_vp, _vp, _vp, _vp, _vp, _f, _i, _i]),
+    "tl_rotary_frequencies": (_i, [_vp, _i, _d, _i, _d, _d, _d, _d]),
+    "tl_rotary_f16": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _i, _i, _f, _i, _i, _i]),
+    "tl_rotary_kv_pages_f16": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _i, _i, _f, _i, _i, _kvp, _vp, _sz, _i]),
+    "tl_paged_attention_workspace": (_sz, [_i, _i, _i, _i, _i]),
+    "tl_paged_attention_f16": (_i, [_vp, _vp, _sz, _kvp, _vp, _sz, _vp, _i, _i, _i, _f, _vp, _sz]),
+    "tl_pages_fork": (_i, [_vp] * 10 + [_i, _i, _i, _i]),
+    "tl_pages_extend": (_i, [_vp] * 5 + [_i, _i, _i, _i]),
+    "tl_pages_free": (_i, [_vp] * 4 + [_i, _i, _i, _i]),
+    "tl_pages_compact": (_i, [_vp] * 8 + [_i, _i, _i]),
+    "tl_pages_copy": (_i, [_vp, _sz, _sz, _sz, _i, _i, _vp, _vp, _vp, _i]),
+    "tl_beam_select_workspace": (_sz, [_i, _i, _i, _i]),
+    "tl_beam_select_f16": (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz]),
+    "tl_beam_advance": (_i, [_vp] * 8 + [_i, _i, _i, _i]),
 }
 
 _lib = None

@@ -14,9 +14,11 @@ import math
 import numpy as np
 import torch
 
-from ._lib import TensorLibError, check, lib
+from ._lib import KvPages, TensorLibError, check, lib
 
 _OPS = {"add": 0, "sub": 1, "mul": 2, "div": 3}
+_ROTARY_LAYOUTS = {"interleaved": 0, "half": 1}
+_ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
 
 
 def _ptr(t: torch.Tensor) -> ctypes.c_void_p:
@@ -486,6 +488,239 @@ class HipDevice:
         check(self.lib.tl_prefill_attention_f16(_ptr(out), _ptr(q), _ptr(cache_k), _ptr(vT), ldv, start_pos, S, H, D),
               "tl_prefill_attention_f16")
         return out
+
+    # -- several sequences over a paged key-value cache --------------------------------
+    def _arg(self, t, dtype, name, shape=None, dense=True):
+        """A tensor of this device with the given type and shape (None: any extent), contiguous if `dense`."""
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise TensorLibError(f"{name} must be a CUDA(HIP) tensor; there is no CPU path")
+        if t.device.index != self.ordinal:
+            raise ValueError(f"{name} is on {t.device}, this device is cuda:{self.ordinal}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if shape is not None and (t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape))):
+            raise ValueError(f"{name} must have shape {tuple('any' if w is None else w for w in shape)}, got {tuple(t.shape)}")
+        if dense and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        return t.data_ptr()
+
+    def _head_rows(self, t, name, heads=None, dim=None):
+        """Pointer and row stride of [rows, heads, dim] halves whose heads lie next to each other (rows may be apart)."""
+        p = self._arg(t, torch.float16, name, (None, heads, dim), dense=False)
+        rows, h, d = t.shape
+        rs, hs, ds = t.stride()
+        if (ds != 1 and d > 1) or (hs != d and h > 1) or (rs < h * d and rows > 1):
+            raise ValueError(f"{name}: the heads of a row must be dense and rows must not overlap, got strides {t.stride()}")
+        return p, rs
+
+    def _kv_pages(self, k_pages, v_pages):
+        pk = self._arg(k_pages, torch.float16, "k_pages", (None, None, None, None), dense=False)
+        pv = self._arg(v_pages, torch.float16, "v_pages", tuple(k_pages.shape), dense=False)
+        n, ps, h, d = k_pages.shape
+        st = k_pages.stride()
+        if v_pages.stride() != st or (st[3] != 1 and d > 1):
+            raise ValueError(f"k_pages and v_pages need equal strides and dense heads, got {st} and {v_pages.stride()}")
+        return KvPages(pk, pv, st[0], st[1], st[2], n, ps, h, d)
+
+    def _may_allocate(self):
+        """Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current
+        stream: the library must enqueue on that one, and launch on this device."""
+        if torch.cuda.current_device() != self.ordinal:
+            raise TensorLibError(f"the current device is cuda:{torch.cuda.current_device()}, this device is cuda:{self.ordinal}")
+        if (self.lib.tl_get_stream() or 0) != torch.cuda.current_stream().cuda_stream:
+            raise TensorLibError("the library stream is not torch's current stream; call bind_stream(torch.cuda.current_stream()) first")
+
+    def rotary_frequencies(self, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                           original_context: float = 0.0, slow_turns: float = 1.0, fast_turns: float = 32.0) -> torch.Tensor:
+        """Radians per position of each pair, float64 on the device; `scaling` is none, linear, base or parts
+        (tl_rotary_frequencies). Computed once per model."""
+        if scaling not in _ROTARY_SCALINGS:
+            raise ValueError(f"unknown scaling {scaling!r}, one of {sorted(_ROTARY_SCALINGS)}")
+        out = np.empty(max(rotary_dim // 2, 1), np.float64)
+        check(self.lib.tl_rotary_frequencies(out.ctypes.data_as(ctypes.c_void_p), rotary_dim, base, _ROTARY_SCALINGS[scaling], factor,
+                                             original_context, slow_turns, fast_turns), "tl_rotary_frequencies")
+        return self.from_numpy(out)
+
+    def rotary(self, x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, layout: str = "half", magnitude: float = 1.0,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """x [tokens, heads, dim] with the first 2 * len(freq) elements of each head rotated to positions[token]; rows may
+        be column blocks of a wider matrix. out=x rotates in place."""
+        px, sx = self._head_rows(x, "x")
+        n, h, d = x.shape
+        if layout not in _ROTARY_LAYOUTS:
+            raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
+        pp, pf = self._arg(positions, torch.int32, "positions", (n,)), self._arg(freq, torch.float64, "freq", (None,))
+        self._may_allocate()
+        if out is None:
+            out = torch.empty((n, h, d), dtype=torch.float16, device=x.device)
+        po, so = self._head_rows(out, "out", h, d)
+        if out.shape[0] != n:
+            raise ValueError(f"out must have {n} rows, got {out.shape[0]}")
+        check(self.lib.tl_rotary_f16(po, so, px, sx, pp, pf, 2 * freq.numel(), _ROTARY_LAYOUTS[layout], magnitude, n, h, d), "tl_rotary_f16")
+        return out
+
+    def rotary_paged(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor | None,
+                     freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, layout: str = "half",
+                     magnitude: float = 1.0, q_out: torch.Tensor | None = None) -> torch.Tensor:
+        """Rotated q [tokens, heads, dim]; rotated k and v [tokens, kv heads, dim] go to the pages [pages, positions, kv heads,
+        dim] that tables [sequences, ..] names for position positions[t] of sequence seq_ids[t] (None: sequence t; -1: a
+        padded token, not stored)."""
+        cache = self._kv_pages(k_pages, v_pages)
+        d = cache.head_dim
+        pq, sq = self._head_rows(q, "q", None, d)
+        n, h, _ = q.shape
+        pk, sk = self._head_rows(k, "k", cache.n_kv_heads, d)
+        pv, sv = self._head_rows(v, "v", cache.n_kv_heads, d)
+        if k.shape[0] != n or v.shape[0] != n:
+            raise ValueError("q, k and v must have the same number of tokens")
+        if layout not in _ROTARY_LAYOUTS:
+            raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
+        pp, pf = self._arg(positions, torch.int32, "positions", (n,)), self._arg(freq, torch.float64, "freq", (None,))
+        ps = None if seq_ids is None else self._arg(seq_ids, torch.int32, "seq_ids", (n,))
+        pt = self._arg(tables, torch.int32, "tables", (None, None))
+        self._may_allocate()
+        if q_out is None:
+            q_out = torch.empty((n, h, d), dtype=torch.float16, device=q.device)
+        po = self._arg(q_out, torch.float16, "q_out", (n, h, d))
+        check(self.lib.tl_rotary_kv_pages_f16(po, pq, sq, pk, sk, pv, sv, pp, ps, pf, 2 * freq.numel(), _ROTARY_LAYOUTS[layout], magnitude, n, h,
+                                              cache, pt, tables.shape[1], tables.shape[0]), "tl_rotary_kv_pages_f16")
+        return q_out
+
+    def paged_attention(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
+                        scale: float | None = None, max_len: int | None = None, out: torch.Tensor | None = None,
+                        workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """One token per sequence: q [sequences, heads, dim] attends to the first lens[b] positions of its pages. max_len
+        bounds lens (default: what the tables cover). The workspace is allocated here unless one is passed (uint8, at
+        least paged_attention_workspace(..) bytes, not shared with a call that may overlap)."""
+        cache = self._kv_pages(k_pages, v_pages)
+        d = cache.head_dim
+        pq, sq = self._head_rows(q, "q", None, d)
+        b, h, _ = q.shape
+        pt, pl = self._arg(tables, torch.int32, "tables", (b, None)), self._arg(lens, torch.int32, "lens", (b,))
+        width = tables.shape[1]
+        if max_len is None:
+            max_len = min(width * cache.page_size, 2 ** 31 - 1)
+        self._may_allocate()
+        if out is None:
+            out = torch.empty((b, h, d), dtype=torch.float16, device=q.device)
+        po = self._arg(out, torch.float16, "out", (b, h, d))
+        need = self.lib.tl_paged_attention_workspace(b, h, cache.n_kv_heads, d, max_len)
+        if workspace is None and need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        pw = None if workspace is None else self._arg(workspace, torch.uint8, "workspace")
+        check(self.lib.tl_paged_attention_f16(po, pq, sq, cache, pt, width, pl, b, h, max_len, 1.0 / math.sqrt(d) if scale is None else scale, pw,
+                                              0 if workspace is None else workspace.numel()), "tl_paged_attention_f16")
+        return out
+
+    def paged_attention_workspace(self, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int) -> int:
+        """Bytes of workspace paged_attention needs for these sizes; 0 where it needs none."""
+        return self.lib.tl_paged_attention_workspace(n_seqs, n_heads, n_kv_heads, head_dim, max_len)
+
+    def _page_state(self, tables, lens, refs):
+        pt = self._arg(tables, torch.int32, "tables", (None, None))
+        return pt, self._arg(lens, torch.int32, "lens", (tables.shape[0],)), self._arg(refs, torch.int32, "refs", (None,))
+
+    def pages_fork(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int):
+        """Row i of the new state continues sequence parents[i] (-1: empty). Returns (tables, lens, refs, copy_src, copy_dst,
+        missing); pages_copy(pool, copy_src, copy_dst) then copies the partly filled pages. missing[0] != 0: not enough
+        free pages, the state is unchanged."""
+        pt, pl, pr = self._page_state(tables, lens, refs)
+        n, width = tables.shape
+        pp = self._arg(parents, torch.int32, "parents", (n,))
+        self._may_allocate()
+        e = lambda *shape: torch.empty(shape, dtype=torch.int32, device=tables.device)  # noqa: E731
+        t, ln, r, src, dst, missing = e(n, width), e(n), e(refs.shape[0]), e(n), e(n), e(1)
+        check(self.lib.tl_pages_fork(pt, pl, pr, pp, t.data_ptr(), ln.data_ptr(), r.data_ptr(), src.data_ptr(), dst.data_ptr(), missing.data_ptr(),
+                                     n, width, refs.shape[0], page_size), "tl_pages_fork")
+        return t, ln, r, src, dst, missing
+
+    def pages_extend(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, add: torch.Tensor, page_size: int) -> torch.Tensor:
+        """Room for add[i] more positions of every sequence, in place. Returns missing ([1]): 0, or why nothing changed."""
+        pt, pl, pr = self._page_state(tables, lens, refs)
+        n, width = tables.shape
+        pa = self._arg(add, torch.int32, "add", (n,))
+        self._may_allocate()
+        missing = torch.empty(1, dtype=torch.int32, device=tables.device)
+        check(self.lib.tl_pages_extend(pt, pl, pr, pa, missing.data_ptr(), n, width, refs.shape[0], page_size), "tl_pages_extend")
+        return missing
+
+    def pages_free(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor, page_size: int) -> None:
+        """Gives back the pages of the sequences with rows[i] true and empties them, in place."""
+        pt, pl, pr = self._page_state(tables, lens, refs)
+        n, width = tables.shape
+        pw = self._arg(rows, torch.bool, "rows", (n,))
+        check(self.lib.tl_pages_free(pt, pl, pr, pw, n, width, refs.shape[0], page_size), "tl_pages_free")
+
+    def pages_compact(self, tables: torch.Tensor, refs: torch.Tensor):
+        """Moves the live pages to the low end of the pool. Returns (tables, refs, remap, copy_src, copy_dst, count);
+        pages_copy(pool, copy_src, copy_dst, count) then moves the data."""
+        pt, pr = self._arg(tables, torch.int32, "tables", (None, None)), self._arg(refs, torch.int32, "refs", (None,))
+        self._may_allocate()
+        n, width = tables.shape
+        pages = refs.shape[0]
+        e = lambda *shape: torch.empty(shape, dtype=torch.int32, device=tables.device)  # noqa: E731
+        t, r, remap, src, dst, count = e(n, width), e(pages), e(pages), e(pages), e(pages), e(1)
+        check(self.lib.tl_pages_compact(pt, pr, t.data_ptr(), r.data_ptr(), remap.data_ptr(), src.data_ptr(), dst.data_ptr(), count.data_ptr(),
+                                        n, width, pages), "tl_pages_compact")
+        return t, r, remap, src, dst, count
+
+    def pages_copy(self, pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, count: torch.Tensor | None = None) -> None:
+        """pool [planes, pages, ..]: page src[i] of every plane to page dst[i], in place; ids of -1 are skipped, and pairs from
+        count[0] on."""
+        if not isinstance(pool, torch.Tensor) or pool.dim() < 3:
+            raise ValueError("pool must be [planes, pages, ...page]")
+        p = self._arg(pool, pool.dtype, "pool", dense=False)
+        item = pool.element_size()
+        planes, pages = pool.shape[:2]
+        if pool.numel() and not pool[0, 0].is_contiguous():
+            raise ValueError("a page of the pool must be contiguous")
+        ps, pd = self._arg(src, torch.int32, "src", (None,)), self._arg(dst, torch.int32, "dst", (src.shape[0],))
+        pc = None if count is None else self._arg(count, torch.int32, "count", (1,))
+        page_bytes = math.prod(pool.shape[2:]) * item
+        check(self.lib.tl_pages_copy(p, pool.stride(0) * item, pool.stride(1) * item, page_bytes, planes, pages, ps, pd, pc, src.shape[0]),
+              "tl_pages_copy")
+
+    def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, n_beams: int, finished: torch.Tensor | None = None, end_token: int = 2,
+                    n_select: int | None = None, workspace: torch.Tensor | None = None):
+        """logits [requests * n_beams, vocab] (rows may be apart), scores (float32) and finished (bool) per row. Returns the best
+        n_select (default n_beams) continuations of every request as flat (scores, tokens, parents), best first."""
+        pl = self._arg(logits, torch.float16, "logits", (None, None), dense=False)
+        rows, vocab = logits.shape
+        if n_beams < 1 or rows % n_beams or logits.stride(1) != 1 and vocab > 1 or logits.stride(0) < vocab and rows > 1:
+            raise ValueError(f"logits must be [requests * {n_beams}, vocab] with dense rows, got {tuple(logits.shape)}, strides {logits.stride()}")
+        ps = self._arg(scores, torch.float32, "scores", (rows,))
+        pf = None if finished is None else self._arg(finished, torch.bool, "finished", (rows,))
+        batch, n = rows // n_beams, n_beams if n_select is None else n_select
+        self._may_allocate()
+        out = torch.empty(max(batch * n, 0), dtype=torch.float32, device=logits.device)
+        tokens, parents = torch.empty_like(out, dtype=torch.int32), torch.empty_like(out, dtype=torch.int32)
+        if workspace is None:
+            workspace = torch.empty(self.lib.tl_beam_select_workspace(batch, n_beams, vocab, n), dtype=torch.uint8, device=logits.device)
+        pw = self._arg(workspace, torch.uint8, "workspace")
+        check(self.lib.tl_beam_select_f16(out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), pl, logits.stride(0), ps, pf, batch, n_beams, vocab, n,
+                                          end_token, pw, workspace.numel()), "tl_beam_select_f16")
+        return out, tokens, parents
+
+    def beam_select_workspace(self, n_batch: int, n_beams: int, vocab: int, n_select: int) -> int:
+        """Bytes of workspace beam_select needs for these sizes."""
+        return self.lib.tl_beam_select_workspace(n_batch, n_beams, vocab, n_select)
+
+    def beam_advance(self, history: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor | None, parents: torch.Tensor,
+                     tokens: torch.Tensor, end_token: int = 2):
+        """The histories [rows, width] after a selection: row i is parents[i]'s with tokens[i] behind it. Returns (history, lens,
+        finished)."""
+        ph = self._arg(history, torch.int32, "history", (None, None))
+        rows, width = history.shape
+        pl = self._arg(lens, torch.int32, "lens", (rows,))
+        pf = None if finished is None else self._arg(finished, torch.bool, "finished", (rows,))
+        pp = self._arg(parents, torch.int32, "parents", (None,))
+        n = parents.shape[0]
+        pt = self._arg(tokens, torch.int32, "tokens", (n,))
+        self._may_allocate()
+        h = torch.empty((n, width), dtype=torch.int32, device=history.device)
+        ln, f = torch.empty(n, dtype=torch.int32, device=history.device), torch.empty(n, dtype=torch.bool, device=history.device)
+        check(self.lib.tl_beam_advance(h.data_ptr(), ln.data_ptr(), f.data_ptr(), ph, pl, pf, pp, pt, rows, n, width, end_token), "tl_beam_advance")
+        return h, ln, f
 
     # -- tuning hooks -------------------------------------------------------------------
     def set_gemv_variant(self, v: int) -> None:

@@ -3,16 +3,23 @@
 //   out[b, h, :] = sum_t p_t V[t, g(h), :] / sum_t p_t,   p_t = exp(scale q.K_t - max),   t < lens[b]
 //
 // Bound by memory: K and V are read once (4 len kv_heads head_dim bytes).  The length is cut into chunks, one workgroup
-// per (sequence, kv head, chunk), four wavefronts that take 32 positions each in turn; more than one chunk leaves fp32
-// partials (max, sum, weighted values) for a second launch to join.  Chunks with no positions leave at once.
+// per (sequence, kv head, chunk), four wavefronts that take 16 or 32 positions each in turn; more than one chunk leaves
+// fp32 partials (max, sum, weighted values) for a second launch to join.  Chunks with no positions leave at once.
 //
-// Both products run on the matrix cores with the query heads of a group as the 16 columns of a tile (a group of one
-// wastes 15 columns, and the matrix cores still have three times the rate that the memory can feed).  The scores are
-// K (16 positions x dims) times Q^T, f16 in, fp32 out: lane (n = lane % 16, g = lane / 16) ends up with head n and
-// positions 4 g + r.  The values then go through the fp32 product, 16 x 4 by 4 x 16, whose operand layouts are exactly
-// that: step r takes position 4 g + r from lane group g, p from the registers that the scores were in, and V converted
-// to fp32 on the way, one dimension of its 16-byte piece per instruction.  No transposition, no LDS round trip, and no
-// rounding of p.
+// Both products run on the matrix cores with the query heads of a group as the 16 columns of a tile; a group of one wastes
+// 15 columns, and the matrix cores are still busy for less than a tenth of the time.  The scores are K (16 positions x
+// dims) times Q^T: lane (n = lane % 16, g = lane / 16) ends up with head n and positions 4 g + r of each tile.  That is
+// what the second product, V^T (dims x positions) times the weights, wants as its right operand, positions being free to
+// stand in any order along k.  For the left one each lane loads 16-byte pieces of exactly those positions of V, and the
+// eight positions of one dimension come together within the lane: no LDS, no exchange between lanes.  A weight goes in
+// as the sum of two halves, 22 bits of it.  (The fp32 product, which takes the weights as they are, has operand
+// layouts that need no exchange at all; its rate made 0.9 us of a 32-position turn: 13.7 against 12.4 us for 1 x 2048
+// positions of 32 heads, 108 against 92 us for 16 x 8000 positions of 256 dims.)
+//
+// Measured (one pass, both launches): 64 sequences of 65 to 4097 positions, 32 heads on 8 of 128: 121 us = 4.6 TB/s; in
+// the middle of the launch the memory runs at 6.0, the rest is the first requests' and the last workgroups' time.
+// 4 sequences of 100001 to 131072, 64 heads on 8: 354 us = 5.4 TB/s.  1 x 2048, 32 heads: 12.5 us, of which the two
+// launches of an empty problem take 8.
 #include <cmath>
 
 #include "paged.h"
@@ -20,10 +27,13 @@
 namespace tl {
 
 constexpr int kWaves = 4;
-constexpr int kTile = 32;                 // positions of a wavefront's turn
-constexpr int kMaxChunk = 2048;           // positions of a workgroup
+constexpr int kMinChunk = 128, kMaxChunk = 1024;   // positions of a workgroup, a power of two
 constexpr int kGroupTile = 16;            // query heads that share a pass over K and V
 constexpr float kLog2e = 1.4426950408889634f;
+// Weights are kept 2^12 times as large as exp(score - max), in the sum too: as halves they lose nothing down to 2^-36 of
+// the largest one.
+constexpr float kWeightLog2 = 12.f;
+constexpr float kTiny = 5.9604644775390625e-8f;   // 2^-24, the smallest positive half
 
 struct PagedAttnArgs {
     half_t* out;
@@ -40,50 +50,55 @@ struct PagedAttnArgs {
     float scale_log2;
 };
 
+// LDS: the offsets of the chunk's positions, then every wavefront's weighted values of every head of the tile.
+template <int DP>
+static size_t attention_lds(int chunk, int group) {
+    return chunk * sizeof(long) + (size_t)kWaves * (group < kGroupTile ? group : kGroupTile) * DP * sizeof(float);
+}
+
+// DP: head_dim rounded up to 64, 128 or 256 (EXACT: equal to it).  U: 16-position tiles per turn of a wavefront; one for
+// DP 256, whose rows fill twice the registers.
 template <int DP, bool EXACT>
-__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel(PagedAttnArgs A) {
+__global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A) {
+    constexpr int U = DP == 256 ? 1 : 2;
+    constexpr int kTile = 16 * U;         // positions of a turn
     constexpr int VD = DP / 16;           // dims of V per lane
     typedef _Float16 vpiece __attribute__((ext_vector_type(VD < 8 ? VD : 8)));
     constexpr int VP = VD / (VD < 8 ? VD : 8);
     constexpr int KJ = DP / 32;
-    __shared__ long s_slot[kMaxChunk];
+    typedef _Float16 weights __attribute__((ext_vector_type(4 * U)));
+    extern __shared__ __align__(16) unsigned char s_dynamic[];
     __shared__ float s_ml[kWaves][2][kGroupTile];
-    __shared__ float s_o[kWaves][kGroupTile][DP];
-    __shared__ int s_bad;
 
     unsigned head_tile, split;
     const unsigned seq = A.by_splits.divmod(A.by_heads.divmod(blockIdx.x, head_tile), split);
-    const int len = A.lens[seq];
     const int t0 = (int)split * A.chunk;
-    // a length beyond what the tables or the caller's bound cover: the first chunk answers NaN for the sequence
-    const bool too_long = len > A.max_len || (size_t)(len > 0 ? (len - 1) / A.cache.page_size : 0) >= A.table_stride;
-    if (split != 0 && (too_long || t0 >= len)) return;
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int col = lane % 16, grp = lane / 16;
     const int kv_head = (int)head_tile / A.group_tiles;
     const int g0 = ((int)head_tile % A.group_tiles) * kGroupTile;
     const int heads = A.group - g0 < kGroupTile ? A.group - g0 : kGroupTile;
     const int head0 = kv_head * A.group + g0;
     const int D = EXACT ? DP : A.cache.head_dim;
-    const int tid = threadIdx.x;
-    if (len <= 0 || too_long) {           // nothing to attend to: zeros
-        const half_t fill = too_long ? (half_t)NAN : (half_t)0.f;
-        half_t* o = A.out + ((size_t)seq * A.n_heads + head0) * D;
-        for (int i = tid; i < heads * D; i += 256) o[i] = fill;
-        return;
-    }
-    const int n = len - t0 < A.chunk ? len - t0 : A.chunk;
-    if (tid == 0) s_bad = 0;
-    __syncthreads();
-    // element offset of every position of the chunk; a page id out of range poisons the result and reads page 0
+    long* s_slot = reinterpret_cast<long*>(s_dynamic) + wave * (A.chunk / kWaves);         // the wavefront's own positions
+    float* s_o = reinterpret_cast<float*>(s_dynamic + A.chunk * sizeof(long));             // [wave][head][DP]
+
+    // The length, the chunk's table entries and the queries are requested together, before any of them is needed.  A
+    // wavefront looks up its own positions only (a turn's of every four), so no barrier stands before its first rows.
     const int* table = A.tables + (size_t)seq * A.table_stride;
-    for (int i = tid; i < n; i += 256) {
-        unsigned row;
-        const unsigned at = A.by_page.divmod((unsigned)(t0 + i), row);
-        int page = table[at];
-        if (page < 0 || page >= A.cache.n_pages) { page = 0; s_bad = 1; }
-        s_slot[i] = (long)((size_t)page * A.cache.page_stride + (size_t)row * A.cache.row_stride);
+    constexpr int LOOKUPS = kMaxChunk / (kWaves * 64);
+    int page[LOOKUPS];
+    unsigned row[LOOKUPS];
+#pragma unroll
+    for (int x = 0; x < LOOKUPS; ++x) {
+        const int i = (x * (64 / kTile) + lane / kTile) * (kWaves * kTile) + wave * kTile + lane % kTile;      // position in the chunk
+        page[x] = 0;
+        row[x] = 0;
+        if (i < A.chunk) {
+            const unsigned at = A.by_page.divmod((unsigned)t0 + (unsigned)i, row[x]);
+            if (at < A.table_stride) page[x] = table[at];
+        }
     }
-    const int lane = tid % 64, wave = tid / 64;
-    const int col = lane % 16, grp = lane / 16;
     // queries: column = head, 8 dims per lane group; columns past the group and dims past the head hold zeros
     half8_t qf[KJ];
     const half8_t zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -92,55 +107,84 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
             const int d = 32 * j + 8 * grp;
-            qf[j] = col < heads && (EXACT || d < D) ? *reinterpret_cast<const half8_t*>(q + (EXACT || d < D ? d : 0)) : zero8;
+            qf[j] = *reinterpret_cast<const half8_t*>(q + (EXACT || d < D ? d : 0));
         }
     }
-    __syncthreads();
+    const int len = A.lens[seq];
+    // a length beyond what the tables or the caller's bound cover: the first chunk answers NaN for the sequence
+    const bool too_long = len > A.max_len || (size_t)(len > 0 ? A.by_page.div((unsigned)len - 1u) : 0u) >= A.table_stride;
+    if (split != 0 && (too_long || t0 >= len)) return;
+    if (len <= 0 || too_long) {           // nothing to attend to: zeros
+        const half_t fill = too_long ? (half_t)NAN : (half_t)0.f;
+        half_t* o = A.out + ((size_t)seq * A.n_heads + head0) * D;
+        for (int i = tid; i < heads * D; i += 256) o[i] = fill;
+        return;
+    }
+    const int n = len - t0 < A.chunk ? len - t0 : A.chunk;
+    // element offsets of the positions; a page id out of range poisons the result and reads page 0
+    bool bad = false;
+#pragma unroll
+    for (int x = 0; x < LOOKUPS; ++x) {
+        const int i = (x * (64 / kTile) + lane / kTile) * (kWaves * kTile) + wave * kTile + lane % kTile;
+        if (page[x] < 0 || page[x] >= A.cache.n_pages) {
+            bad |= i < n;
+            page[x] = 0;
+        }
+        if (i < A.chunk)
+            s_slot[x * 64 + lane] = (long)((size_t)page[x] * A.cache.page_stride + (size_t)row[x] * A.cache.row_stride);
+    }
+    bad = __any(bad);
+#pragma unroll
+    for (int j = 0; j < KJ; ++j)
+        if (col >= heads || (!EXACT && 32 * j + 8 * grp >= D)) qf[j] = zero8;
 
     const half_t* kbase = static_cast<const half_t*>(A.cache.k) + (size_t)kv_head * A.cache.head_stride;
     const half_t* vbase = static_cast<const half_t*>(A.cache.v) + (size_t)kv_head * A.cache.head_stride;
-    half8_t kf[2][KJ];
-    vpiece vf[2][4][VP];
-    auto load_k = [&](int t) {
+    half8_t kf[U][KJ];
+    vpiece vf[U][4][VP];
+    // Rows of the wavefront's turn `s` (16 U positions).  Positions behind the end read what their table entry names, page
+    // 0 if it names none: inside the cache in any case.  The fences keep the requests where they stand: the compiler
+    // would move those of the next turn's V behind the wait for its K.
+    auto load_k = [&](int s) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int i = t + 16 * u + col;
-            const half_t* p = kbase + s_slot[i < n ? i : n - 1];
+        for (int u = 0; u < U; ++u) {
+            const half_t* p = kbase + s_slot[s * kTile + 16 * u + col];
 #pragma unroll
             for (int j = 0; j < KJ; ++j) {
                 const int d = 32 * j + 8 * grp;
                 kf[u][j] = *reinterpret_cast<const half8_t*>(p + (EXACT || d < D ? d : 0));
             }
         }
+        asm volatile("" ::: "memory");
     };
-    auto load_v = [&](int t) {
+    auto load_v = [&](int s) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = t + 16 * u + 4 * grp + r;
-                const half_t* p = vbase + s_slot[i < n ? i : n - 1];
+                const half_t* p = vbase + s_slot[s * kTile + 16 * u + 4 * grp + r];
 #pragma unroll
                 for (int x = 0; x < VP; ++x) {
                     const int d = col * VD + 8 * x;
                     vf[u][r][x] = *reinterpret_cast<const vpiece*>(p + (EXACT || d < D ? d : 0));
                 }
             }
+        asm volatile("" ::: "memory");
     };
 
     float4_t acc[VD];
 #pragma unroll
     for (int i = 0; i < VD; ++i) acc[i] = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;         // running maximum (whole column) and this lane's share of the sum
-    int t = wave * kTile;
+    int t = wave * kTile, turn = 0;
     if (t < n) {
-        load_k(t);
-        load_v(t);
+        load_k(0);
+        load_v(0);
     }
-    for (; t < n; t += kWaves * kTile) {
-        float4_t sc[2];
+    for (; t < n; t += kWaves * kTile, ++turn) {
+        float4_t sc[U];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
             sc[u] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < KJ; ++j) {
@@ -150,11 +194,11 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel
             }
         }
         const int next = t + kWaves * kTile;
-        if (next < n) load_k(next);
-        float p[2][4];
+        if (next < n) load_k(turn + 1);
+        float p[U][4];
         float mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 p[u][r] = t + 16 * u + 4 * grp + r < n ? sc[u][r] * A.scale_log2 : -INFINITY;
@@ -170,15 +214,15 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel
 #pragma unroll
         for (int i = 0; i < VD; ++i) acc[i] *= alpha;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                p[u][r] = __builtin_amdgcn_exp2f(p[u][r] - base);
+                p[u][r] = __builtin_amdgcn_exp2f(p[u][r] - base + kWeightLog2);
                 l += p[u][r];
             }
         if (t + kTile > n) {              // what lies behind the end may hold anything, and 0 times it must be 0
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (t + 16 * u + 4 * grp + r >= n) {
@@ -186,14 +230,35 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel
                         for (int x = 0; x < VP; ++x) vf[u][r][x] = (vpiece)(half_t)0.f;
                     }
         }
+        // p as the sum of two halves: no bit of it that matters is lost.  hi is rounded towards zero and neither part of a
+        // positive weight becomes zero, so that an infinite value keeps its sign.  The eight (four) positions of a lane
+        // come together as A[row = dims, k = position] by exchanges within the lane.
+        weights hi, lo;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r) {
+                const float x = p[u][r], tiny = x > 0.f ? kTiny : 0.f;
+                const half_t h = (half_t)__builtin_amdgcn_cvt_pkrtz(fmaxf(x, tiny), 0.f)[0];
+                hi[4 * u + r] = h;
+                lo[4 * u + r] = (half_t)fmaxf(x - (float)h, tiny);
+            }
 #pragma unroll
-                for (int i = 0; i < VD; ++i)
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)vf[u][r][i / 8][i % 8], p[u][r], acc[i], 0, 0, 0);
-        if (next < n) load_v(next);
+        for (int i = 0; i < VD; ++i) {
+            weights a;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a[4 * u + r] = vf[u][r][i / 8][i % 8];
+            if constexpr (U == 2) {
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi, acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo, acc[i], 0, 0, 0);
+            } else {
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, hi, acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, lo, acc[i], 0, 0, 0);
+            }
+        }
+        if (next < n) load_v(turn + 1);
     }
 
     // join the wavefronts: lane (col, grp) holds head col, dims (4 grp + r) * VD + i
@@ -201,13 +266,13 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel
     l += __shfl_xor(l, 32, 64);
     if (grp == 0) {
         s_ml[wave][0][col] = m;
-        s_ml[wave][1][col] = l;
+        s_ml[wave][1][col] = bad ? NAN : l;
     }
     if (col < heads) {
 #pragma unroll
         for (int i = 0; i < VD; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s_o[wave][col][(4 * grp + r) * VD + i] = acc[i][r];
+            for (int r = 0; r < 4; ++r) s_o[(wave * heads + col) * DP + (4 * grp + r) * VD + i] = acc[i][r];
     }
     __syncthreads();
     const bool whole = len <= A.chunk;    // the only chunk: the result itself
@@ -223,11 +288,10 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel
         float sum = 0.f, o = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - top);
+            const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - top);   // 0 * NaN stays NaN
             sum += f * s_ml[w][1][h];
-            o += f * s_o[w][h][d];
+            o += f * s_o[(w * heads + h) * DP + d];
         }
-        if (s_bad) sum = NAN;
         if (whole) {
             A.out[((size_t)seq * A.n_heads + head0) * D + i] = (half_t)(o / sum);
         } else {
@@ -237,40 +301,87 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) paged_attention_kernel
     }
 }
 
-// Joins the chunks of one (head, sequence): D threads, the chunks in order.
-__global__ void __launch_bounds__(256) paged_attention_join_kernel(PagedAttnArgs A) {
-    const int h = blockIdx.x, seq = blockIdx.y, D = A.cache.head_dim, d = threadIdx.x;
+// Joins the chunks of one (head, sequence): D / 4 threads take four dims each of every n-th chunk, several chunks' loads in
+// flight together (a dependent load per chunk would cost a memory latency each), then the groups of threads join in LDS.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_attention_join_kernel(PagedAttnArgs A) {
+    constexpr int U = 8;
+    __shared__ float4_t s_o[THREADS];
+    __shared__ float s_m[THREADS], s_l[THREADS];
+    const int h = blockIdx.x, seq = blockIdx.y, D = A.cache.head_dim;
     const int len = A.lens[seq];
     if (len <= A.chunk || len > A.max_len || (size_t)((len - 1) / A.cache.page_size) >= A.table_stride) return;
     const int n = (len + A.chunk - 1) / A.chunk;
-    if (d >= D) return;
+    const int per = D / 4, groups = THREADS / per;
+    const int grp = threadIdx.x / per, d = (threadIdx.x % per) * 4;
     const size_t part = (size_t)seq * A.n_splits * A.n_heads + h;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int i = 0; i < n; ++i) {
-        const float2 ml = A.part_ml[part + (size_t)i * A.n_heads];
-        const float x = A.part_o[(part + (size_t)i * A.n_heads) * D + d];
-        const float m_new = fmaxf(m, ml.x);
-        const float base = m_new == -INFINITY ? 0.f : m_new;
-        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(ml.x - base);
-        l = l * f0 + ml.y * f1;
-        o = o * f0 + x * f1;
-        m = m_new;
+    float m = -INFINITY, l = 0.f;
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+    if (grp < groups) {
+        for (int i0 = grp; i0 < n; i0 += U * groups) {
+            float2 ml[U];
+            float4_t x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * groups;
+                const size_t at = part + (size_t)(i < n ? i : i0) * A.n_heads;
+                ml[u] = A.part_ml[at];
+                x[u] = *reinterpret_cast<const float4_t*>(A.part_o + at * D + d);
+                if (i >= n) ml[u].x = -INFINITY;
+            }
+            float m_new = m;
+#pragma unroll
+            for (int u = 0; u < U; ++u) m_new = fmaxf(m_new, ml[u].x);
+            const float base = m_new == -INFINITY ? 0.f : m_new;
+            const float f0 = __builtin_amdgcn_exp2f(m - base);
+            l *= f0;
+            o *= f0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i0 + u * groups >= n) break;
+                const float f = __builtin_amdgcn_exp2f(ml[u].x - base);
+                l += ml[u].y * f;
+                o += x[u] * f;
+            }
+            m = m_new;
+        }
     }
-    A.out[((size_t)seq * A.n_heads + h) * D + d] = (half_t)(o / l);
+    s_m[threadIdx.x] = m;
+    s_l[threadIdx.x] = l;
+    s_o[threadIdx.x] = o;
+    __syncthreads();
+    if (grp != 0) return;
+    for (int g = 1; g < groups; ++g) m = fmaxf(m, s_m[threadIdx.x + g * per]);
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    o = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < groups; ++g) {
+        const float f = __builtin_amdgcn_exp2f(s_m[threadIdx.x + g * per] - base);
+        l += s_l[threadIdx.x + g * per] * f;
+        o += s_o[threadIdx.x + g * per] * f;
+    }
+    half4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (half_t)(o[i] / l);
+    *reinterpret_cast<half4_t*>(A.out + ((size_t)seq * A.n_heads + h) * D + d) = r;
 }
 
-// Positions per workgroup: as many as leave about four workgroups per compute unit (256 of them).
+// Positions per workgroup.  512: a workgroup then lives for 20 us in a saturated memory system, and the last ones of a
+// ragged batch end close together (64 sequences of 65 to 4097 positions, 32 heads on 8: 121 us, against 134 with 2048 and
+// 132 with 128).  1024 for long contexts, where the partials are what can be saved (4 x 131072: 352 against 362 us).
+// Fewer as long as there are not four workgroups per compute unit (1 x 32768: 38 us with 256, 40 with 128, 47 with 1024).
 static int chunk_of(int n_seqs, int head_tiles, int max_len) {
-    int chunk = kMaxChunk;
-    while (chunk > kWaves * kTile && (double)n_seqs * head_tiles * ((max_len + (double)chunk - 1) / chunk) < 1024.0) chunk /= 2;
+    int chunk = max_len > 32768 ? kMaxChunk : kMaxChunk / 2;
+    while (chunk > kMinChunk && (double)n_seqs * head_tiles * ((max_len + (double)chunk - 1) / chunk) < 1024.0) chunk /= 2;
     return chunk;
 }
 static int group_tiles_of(int n_heads, int n_kv_heads) { return (n_heads / n_kv_heads + kGroupTile - 1) / kGroupTile; }
 
 template <int DP>
 static void launch_paged_attention(const PagedAttnArgs& A, unsigned blocks) {
-    if (A.cache.head_dim == DP) paged_attention_kernel<DP, true><<<blocks, 256, 0, stream()>>>(A);
-    else paged_attention_kernel<DP, false><<<blocks, 256, 0, stream()>>>(A);
+    const size_t lds = attention_lds<DP>(A.chunk, A.group);
+    if (A.cache.head_dim == DP) paged_attention_kernel<DP, true><<<blocks, 256, lds, stream()>>>(A);
+    else paged_attention_kernel<DP, false><<<blocks, 256, lds, stream()>>>(A);
 }
 
 }  // namespace tl
@@ -295,6 +406,7 @@ int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_k
     TL_REQUIRE(std::isfinite(scale), "%s: scale must be finite", what);
     if (n_seqs == 0) return TL_OK;
     TL_REQUIRE(out && q && lens && (tables || table_stride == 0), "%s: null pointer", what);
+    TL_REQUIRE((reinterpret_cast<uintptr_t>(out) & 7u) == 0, "%s: the output must be 8-byte aligned", what);
     TL_REQUIRE(aligned16(q) && (n_seqs == 1 || q_stride % 8 == 0), "%s: query rows must be 16-byte aligned", what);
     TL_REQUIRE(n_seqs == 1 || q_stride >= (size_t)n_heads * cache->head_dim, "%s: the query stride must cover the heads", what);
     PagedAttnArgs A{};
@@ -319,8 +431,8 @@ int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_k
     A.tables = tables;
     A.table_stride = table_stride;
     A.lens = lens;
-    A.part_ml = static_cast<float2*>(workspace);
-    A.part_o = static_cast<float*>(workspace) + 2 * parts;
+    A.part_o = static_cast<float*>(workspace);
+    A.part_ml = reinterpret_cast<float2*>(A.part_o + parts * cache->head_dim);
     A.by_page = FastDiv((unsigned)cache->page_size);
     A.by_heads = FastDiv((unsigned)head_tiles);
     A.by_splits = FastDiv((unsigned)A.n_splits);
@@ -332,7 +444,10 @@ int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_k
     else launch_paged_attention<256>(A, (unsigned)blocks);
     TL_CHECK_LAUNCH("paged_attention_kernel");
     if (A.n_splits > 1) {
-        paged_attention_join_kernel<<<dim3(n_heads, n_seqs), cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256, 0, stream()>>>(A);
+        // 256 threads where they cover the chunks in one round trip (16 x 8000 positions of 64 dims: 22 us, 24 with 1024),
+        // else 1024 (1 x 32768 in 256 chunks: 40 us, 45 with 256)
+        if (A.n_splits <= 8 * (256 / (cache->head_dim / 4))) paged_attention_join_kernel<256><<<dim3(n_heads, n_seqs), 256, 0, stream()>>>(A);
+        else paged_attention_join_kernel<1024><<<dim3(n_heads, n_seqs), 1024, 0, stream()>>>(A);
         TL_CHECK_LAUNCH("paged_attention_join_kernel");
     }
     return TL_OK;

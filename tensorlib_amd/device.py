@@ -491,18 +491,20 @@ class HipDevice:
 
     # -- several sequences over a paged key-value cache --------------------------------
     def _arg(self, t, dtype, name, shape=None, dense=True):
-        """A tensor of this device with the given type and shape (None: any extent), contiguous if `dense`."""
+        """Pointer of a tensor of this device with the given type and shape (None: any extent), contiguous if `dense`.
+        These checks run in front of kernels of a few microseconds, hence the one expression for what is right."""
+        if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self.ordinal and (not dense or t.is_contiguous())
+                and (shape is None or (len(shape) == t.dim() and all([w is None or w == g for w, g in zip(shape, t.shape)])))):
+            return t.data_ptr()
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise TensorLibError(f"{name} must be a CUDA(HIP) tensor; there is no CPU path")
         if t.device.index != self.ordinal:
             raise ValueError(f"{name} is on {t.device}, this device is cuda:{self.ordinal}")
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
         if shape is not None and (t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape))):
             raise ValueError(f"{name} must have shape {tuple('any' if w is None else w for w in shape)}, got {tuple(t.shape)}")
-        if dense and not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-        return t.data_ptr()
+        raise ValueError(f"{name} must be contiguous")
 
     def _head_rows(self, t, name, heads=None, dim=None):
         """Pointer and row stride of [rows, heads, dim] halves whose heads lie next to each other (rows may be apart)."""
@@ -525,9 +527,9 @@ class HipDevice:
     def _may_allocate(self):
         """Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current
         stream: the library must enqueue on that one, and launch on this device."""
-        if torch.cuda.current_device() != self.ordinal:
+        if torch._C._cuda_getDevice() != self.ordinal:
             raise TensorLibError(f"the current device is cuda:{torch.cuda.current_device()}, this device is cuda:{self.ordinal}")
-        if (self.lib.tl_get_stream() or 0) != torch.cuda.current_stream().cuda_stream:
+        if (self.lib.tl_get_stream() or 0) != torch._C._cuda_getCurrentRawStream(self.ordinal):
             raise TensorLibError("the library stream is not torch's current stream; call bind_stream(torch.cuda.current_stream()) first")
 
     def rotary_frequencies(self, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -616,6 +618,12 @@ class HipDevice:
         """Bytes of workspace paged_attention needs for these sizes; 0 where it needs none."""
         return self.lib.tl_paged_attention_workspace(n_seqs, n_heads, n_kv_heads, head_dim, max_len)
 
+    @staticmethod
+    def _int_arrays(like, *sizes):
+        """int32 arrays of these sizes out of one allocation, each 16-byte aligned."""
+        room = [(n + 3) & ~3 for n in sizes]
+        return [t if t.shape[0] == n else t[:n] for t, n in zip(like.new_empty(sum(room)).split(room), sizes)]
+
     def _page_state(self, tables, lens, refs):
         pt = self._arg(tables, torch.int32, "tables", (None, None))
         return pt, self._arg(lens, torch.int32, "lens", (tables.shape[0],)), self._arg(refs, torch.int32, "refs", (None,))
@@ -628,8 +636,8 @@ class HipDevice:
         n, width = tables.shape
         pp = self._arg(parents, torch.int32, "parents", (n,))
         self._may_allocate()
-        e = lambda *shape: torch.empty(shape, dtype=torch.int32, device=tables.device)  # noqa: E731
-        t, ln, r, src, dst, missing = e(n, width), e(n), e(refs.shape[0]), e(n), e(n), e(1)
+        t, ln, r, src, dst, missing = self._int_arrays(tables, n * width, n, refs.shape[0], n, n, 1)
+        t = t.view(n, width)
         check(self.lib.tl_pages_fork(pt, pl, pr, pp, t.data_ptr(), ln.data_ptr(), r.data_ptr(), src.data_ptr(), dst.data_ptr(), missing.data_ptr(),
                                      n, width, refs.shape[0], page_size), "tl_pages_fork")
         return t, ln, r, src, dst, missing
@@ -640,7 +648,7 @@ class HipDevice:
         n, width = tables.shape
         pa = self._arg(add, torch.int32, "add", (n,))
         self._may_allocate()
-        missing = torch.empty(1, dtype=torch.int32, device=tables.device)
+        missing = tables.new_empty(1)
         check(self.lib.tl_pages_extend(pt, pl, pr, pa, missing.data_ptr(), n, width, refs.shape[0], page_size), "tl_pages_extend")
         return missing
 
@@ -658,8 +666,8 @@ class HipDevice:
         self._may_allocate()
         n, width = tables.shape
         pages = refs.shape[0]
-        e = lambda *shape: torch.empty(shape, dtype=torch.int32, device=tables.device)  # noqa: E731
-        t, r, remap, src, dst, count = e(n, width), e(pages), e(pages), e(pages), e(pages), e(1)
+        t, r, remap, src, dst, count = self._int_arrays(tables, n * width, pages, pages, pages, pages, 1)
+        t = t.view(n, width)
         check(self.lib.tl_pages_compact(pt, pr, t.data_ptr(), r.data_ptr(), remap.data_ptr(), src.data_ptr(), dst.data_ptr(), count.data_ptr(),
                                         n, width, pages), "tl_pages_compact")
         return t, r, remap, src, dst, count

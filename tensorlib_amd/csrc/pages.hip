@@ -89,15 +89,223 @@ __device__ void take_free(int* refs, int n_pages, int wanted, F take) {
     }
 }
 
-__global__ void __launch_bounds__(256) pages_copy_ints_kernel(int* out, const int* in, size_t n) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) out[i] = in[i];
-}
+// ---- states that fit one workgroup: the whole operation in one launch, the reference counts in registers or LDS ----
+
+constexpr int kPer = 16;                   // pages per thread
+constexpr int kSmallPages = kPer * kThreads;
+constexpr int kSmallSeqs = kThreads;       // a thread per row
+constexpr size_t kSmallEntries = 65536;    // table entries
+
+// The thread's pages [16 tid, 16 tid + 16); pages past the end count as taken.
+struct MyPages {
+    int ref[kPer];
+    __device__ __forceinline__ void load(const int* refs, int n_pages) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int p = (int)threadIdx.x * kPer + j;
+            ref[j] = p < n_pages ? refs[p] : 1;
+        }
+    }
+    __device__ __forceinline__ int free_count() const {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) n += ref[j] == 0;
+        return n;
+    }
+    // Takes those of the thread's free pages whose rank in page order, from `rank` on, is below `wanted`.
+    template <class F>
+    __device__ __forceinline__ void take(int rank, int wanted, F give) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (ref[j] != 0) continue;
+            if (rank < wanted) {
+                ref[j] = 1;
+                give(rank, (int)threadIdx.x * kPer + j);
+            }
+            ++rank;
+        }
+    }
+};
 
 struct ForkArgs {
     const int *tables, *lens, *refs, *parents;
     int *tables_out, *lens_out, *refs_out, *copy_src, *copy_dst, *missing;
     int n_seqs, table_stride, n_pages, page_size;
+    FastDiv by_vectors;                    // table entries of a row, in steps of VEC
 };
+
+// VEC: table entries a thread moves at a time, 4 where rows are 16-byte aligned.
+template <int VEC>
+__global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) {
+    __shared__ int s_len[kSmallSeqs], s_parent[kSmallSeqs], s_first[kSmallSeqs], s_page[kSmallSeqs];
+    extern __shared__ int s_refs[];
+    const int r = threadIdx.x;
+    const bool row = r < A.n_seqs;
+    const int parent = row ? A.parents[r] : -1;
+    const int old_len = row ? A.lens[r] : 0;
+    for (int p = r; p < A.n_pages; p += kThreads) s_refs[p] = A.refs[p];
+    s_first[r] = kSmallSeqs;
+    s_len[r] = old_len > 0 ? old_len : 0;
+    s_parent[r] = parent >= 0 && parent < A.n_seqs ? parent : -1;
+    __syncthreads();
+    const bool has = s_parent[r] >= 0;
+    const int len = has ? s_len[parent] : 0;
+    const int new_pages = pages_of(len, A.page_size, A.table_stride);
+    const bool partial = len % A.page_size != 0;
+    int last = -1;                         // the page to be copied, if the row is not its parent's first
+    if (partial) {
+        last = A.tables[(size_t)parent * A.table_stride + new_pages - 1];
+        atomicMin(s_first + parent, r);
+    }
+    __syncthreads();
+    const bool copied = partial && s_first[parent] != r;
+    if (copied) s_page[r] = -2;            // not counted and not written below
+    else s_page[r] = -1;
+    __syncthreads();
+    const unsigned total = (unsigned)A.n_seqs * A.by_vectors.d;
+    for (unsigned i = r; i < total; i += kThreads) {
+        unsigned c;
+        const unsigned to = A.by_vectors.divmod(i, c);
+        c *= VEC;
+        const int from = s_parent[to];
+        const int old_pages = pages_of(s_len[to], A.page_size, A.table_stride);
+        const int pages = from >= 0 ? pages_of(s_len[from], A.page_size, A.table_stride) : 0;
+        const int kept = s_page[to] == -2 ? pages - 1 : pages;
+        int o[VEC], x[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            o[j] = -1;
+            x[j] = -1;
+        }
+        const int* old_row = A.tables + (size_t)to * A.table_stride + c;
+        const int* new_row = A.tables + (size_t)(from >= 0 ? from : 0) * A.table_stride + c;
+        if constexpr (VEC == 4) {
+            if ((int)c < old_pages) *reinterpret_cast<int4*>(o) = *reinterpret_cast<const int4*>(old_row);
+            if ((int)c < pages) *reinterpret_cast<int4*>(x) = *reinterpret_cast<const int4*>(new_row);
+        } else {
+            if ((int)c < old_pages) o[0] = *old_row;
+            if ((int)c < pages) x[0] = *new_row;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if ((int)c + j < old_pages && o[j] >= 0 && o[j] < A.n_pages) atomicSub(s_refs + o[j], 1);
+            if ((int)c + j >= pages) x[j] = -1;
+            if ((int)c + j < kept && x[j] >= 0 && x[j] < A.n_pages) atomicAdd(s_refs + x[j], 1);
+        }
+        int* out = A.tables_out + (size_t)to * A.table_stride + c;
+        if constexpr (VEC == 4) *reinterpret_cast<int4*>(out) = *reinterpret_cast<int4*>(x);
+        else *out = x[0];
+    }
+    __syncthreads();
+    const bool wants = copied && last >= 0 && last < A.n_pages;
+    int wanted, available;
+    const int rank = block_scan(wants, &wanted);
+    MyPages mine;
+    mine.load(s_refs, A.n_pages);
+    const int before = block_scan(mine.free_count(), &available);
+    const bool enough = available >= wanted;
+    if (enough) mine.take(before, wanted, [&](int k, int page) {
+        s_page[k] = page;
+        s_refs[page] = 1;
+    });
+    __syncthreads();
+    if (r == 0) *A.missing = enough ? 0 : wanted - available;
+    if (row) {
+        const int page = wants && enough ? s_page[rank] : -1;
+        if (page >= 0) A.tables_out[(size_t)r * A.table_stride + new_pages - 1] = page;
+        A.copy_src[r] = page >= 0 ? last : -1;
+        A.copy_dst[r] = page;
+        A.lens_out[r] = enough ? len : old_len;
+    }
+    for (int p = r; p < A.n_pages; p += kThreads) A.refs_out[p] = enough ? s_refs[p] : A.refs[p];
+    if (!enough)
+        for (size_t i = r; i < (size_t)A.n_seqs * A.table_stride; i += kThreads) A.tables_out[i] = A.tables[i];
+}
+
+__global__ void __launch_bounds__(kThreads)
+pages_extend_small_kernel(int* tables, int* lens, int* refs, const int* add, int* missing, int n_seqs, int table_stride, int n_pages, int page_size) {
+    __shared__ int s_first[kSmallSeqs];   // number of pages wanted by the rows before
+    const int r = threadIdx.x;
+    const int len = r < n_seqs ? max(lens[r], 0) : 0;
+    const long more = r < n_seqs ? max(add[r], 0) : 0;
+    MyPages mine;
+    mine.load(refs, n_pages);
+    const long pages = (len + more + page_size - 1) / page_size;
+    const bool fits = pages <= table_stride && len + more <= 0x7fffffffl;
+    const int held = pages_of(len, page_size, table_stride);
+    int wanted, available;
+    s_first[r] = block_scan(fits ? (int)pages - held : 0, &wanted);
+    const int before = block_scan(mine.free_count(), &available);
+    const bool refused = __syncthreads_or(!fits);
+    if (r == 0) *missing = refused ? -1 : available < wanted ? wanted - available : 0;
+    if (refused || available < wanted) return;
+    mine.take(before, wanted, [&](int k, int page) {
+        int lo = 0, hi = n_seqs - 1;      // the last row whose first page is at most k
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (s_first[mid] <= k) lo = mid;
+            else hi = mid - 1;
+        }
+        refs[page] = 1;
+        tables[(size_t)lo * table_stride + pages_of(lens[lo], page_size, table_stride) + k - s_first[lo]] = page;
+    });
+    __syncthreads();                       // every length has been read
+    if (r < n_seqs) lens[r] = len + (int)more;
+}
+
+// Plan and remap of a small pool.  s_new: a page's new id; the k-th mover and the k-th hole meet in the two lists.
+__global__ void __launch_bounds__(kThreads)
+pages_compact_small_kernel(const int* tables, const int* refs, int* tables_out, int* refs_out, int* remap, int* copy_src, int* copy_dst, int* count,
+                           int n_pages, int n_entries) {
+    __shared__ unsigned short s_mover[kSmallPages / 2], s_hole[kSmallPages / 2];
+    extern __shared__ int s_new[];
+    const int tid = threadIdx.x;
+    MyPages mine;
+    mine.load(refs, n_pages);
+    int live = 0, n = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) n += tid * kPer + j < n_pages && mine.ref[j] > 0;
+    block_scan(n, &live);
+    int movers = 0, holes = 0, total;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int p = tid * kPer + j;
+        movers += p < n_pages && p >= live && mine.ref[j] > 0;
+        holes += p < live && mine.ref[j] <= 0;
+    }
+    int m = block_scan(movers, &total), h = block_scan(holes, &holes);
+    movers = total;                        // as many as holes, at most half of the pages
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int p = tid * kPer + j;
+        if (p >= n_pages) break;
+        if (p >= live && mine.ref[j] > 0) s_mover[m++] = (unsigned short)p;
+        if (p < live && mine.ref[j] <= 0) s_hole[h++] = (unsigned short)p;
+        s_new[p] = mine.ref[j] > 0 ? p : -1;
+    }
+    __syncthreads();
+    for (int k = tid; k < movers; k += kThreads) s_new[s_mover[k]] = s_hole[k];
+    __syncthreads();
+    for (int k = tid; k < n_pages; k += kThreads) {
+        copy_src[k] = k < movers ? s_mover[k] : -1;
+        copy_dst[k] = k < movers ? s_hole[k] : -1;
+        const int to = s_new[k], ref = refs[k];
+        remap[k] = to;
+        if (k >= live) refs_out[k] = 0;
+        if (to >= 0) refs_out[to] = ref;   // below the line: itself, or the hole that it fills
+    }
+    if (tid == 0) *count = movers;
+    for (int i = tid; i < n_entries; i += kThreads) {
+        const int p = tables[i];
+        tables_out[i] = p >= 0 && p < n_pages ? s_new[p] : p;
+    }
+}
+
+// ---- any size ----
+
+__global__ void __launch_bounds__(256) pages_copy_ints_kernel(int* out, const int* in, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) out[i] = in[i];
+}
 
 // One workgroup per row: releases the row's old pages, takes its parent's, and notes the page to be copied for a child
 // after the first of a parent with a partly filled page.
@@ -310,6 +518,10 @@ static int check_state(const char* what, int n_seqs, int table_stride, int n_pag
     return TL_OK;
 }
 
+static bool small_state(int n_seqs, int table_stride, int n_pages) {
+    return n_seqs <= kSmallSeqs && n_pages <= kSmallPages && (size_t)n_seqs * (size_t)table_stride <= kSmallEntries;
+}
+
 static unsigned ints_grid(size_t n) {
     const size_t b = (n + 255) / 256;
     return (unsigned)(b < 2048 ? b : 2048);
@@ -329,7 +541,15 @@ int tl_pages_fork(const int* tables, const int* lens, const int* refs, const int
     TL_REQUIRE(n_seqs == 0 || (tables && lens && parents && tables_out && lens_out && copy_src && copy_dst), "%s: null pointer", what);
     TL_REQUIRE(tables_out != tables && lens_out != lens && refs_out != refs, "%s: the new state must not lie over the old one", what);
     TL_ENSURE_INIT();
-    ForkArgs A{tables, lens, refs, parents, tables_out, lens_out, refs_out, copy_src, copy_dst, missing, n_seqs, table_stride, n_pages, page_size};
+    ForkArgs A{tables, lens, refs, parents, tables_out, lens_out, refs_out, copy_src, copy_dst, missing, n_seqs, table_stride, n_pages, page_size, {}};
+    if (small_state(n_seqs, table_stride, n_pages)) {
+        const bool vec = table_stride % 4 == 0 && aligned16(tables) && aligned16(tables_out);
+        A.by_vectors = FastDiv((unsigned)(vec ? table_stride / 4 : table_stride));
+        if (vec) pages_fork_small_kernel<4><<<1, kThreads, n_pages * sizeof(int), stream()>>>(A);
+        else pages_fork_small_kernel<1><<<1, kThreads, n_pages * sizeof(int), stream()>>>(A);
+        TL_CHECK_LAUNCH("pages_fork_small_kernel");
+        return TL_OK;
+    }
     pages_copy_ints_kernel<<<ints_grid(n_pages), 256, 0, stream()>>>(refs_out, refs, n_pages);
     TL_CHECK_LAUNCH("pages_copy_ints_kernel");
     if (n_seqs > 0) {
@@ -348,6 +568,11 @@ int tl_pages_extend(int* tables, int* lens, int* refs, const int* add, int* miss
     if (rc != TL_OK) return rc;
     TL_REQUIRE(refs && missing && (n_seqs == 0 || (tables && lens && add)), "%s: null pointer", what);
     TL_ENSURE_INIT();
+    if (small_state(n_seqs, 1, n_pages)) {
+        pages_extend_small_kernel<<<1, kThreads, 0, stream()>>>(tables, lens, refs, add, missing, n_seqs, table_stride, n_pages, page_size);
+        TL_CHECK_LAUNCH("pages_extend_small_kernel");
+        return TL_OK;
+    }
     pages_extend_kernel<<<1, kThreads, (size_t)n_seqs * sizeof(int), stream()>>>(tables, lens, refs, add, missing, n_seqs, table_stride, n_pages, page_size);
     TL_CHECK_LAUNCH("pages_extend_kernel");
     return TL_OK;
@@ -374,6 +599,12 @@ int tl_pages_compact(const int* tables, const int* refs, int* tables_out, int* r
     TL_REQUIRE(refs && refs_out && remap && copy_src && copy_dst && count && (n_seqs == 0 || (tables && tables_out)), "%s: null pointer", what);
     TL_REQUIRE(refs_out != refs, "%s: the new reference counts must not lie over the old ones", what);
     TL_ENSURE_INIT();
+    if (small_state(0, 1, n_pages) && (size_t)n_seqs * (size_t)table_stride <= kSmallEntries) {
+        pages_compact_small_kernel<<<1, kThreads, n_pages * sizeof(int), stream()>>>(tables, refs, tables_out, refs_out, remap, copy_src, copy_dst, count,
+                                                                                    n_pages, n_seqs * table_stride);
+        TL_CHECK_LAUNCH("pages_compact_small_kernel");
+        return TL_OK;
+    }
     pages_compact_plan_kernel<<<1, kThreads, 0, stream()>>>(refs, refs_out, remap, copy_src, copy_dst, count, n_pages);
     TL_CHECK_LAUNCH("pages_compact_plan_kernel");
     const size_t n = (size_t)n_seqs * table_stride;

@@ -490,39 +490,49 @@ class HipDevice:
         return out
 
     # -- several sequences over a paged key-value cache --------------------------------
-    def _arg(self, t, dtype, name, shape=None, dense=True):
-        """Pointer of a tensor of this device with the given type and shape (None: any extent), contiguous if `dense`.
-        These checks run in front of kernels of a few microseconds, hence the one expression for what is right."""
-        if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self.ordinal and (not dense or t.is_contiguous())
-                and (shape is None or (len(shape) == t.dim() and all([w is None or w == g for w, g in zip(shape, t.shape)])))):
-            return t.data_ptr()
+    # The checks below stand in front of kernels of a few microseconds: one expression each for what is right, and
+    # _refuse() to say what is wrong.
+    def _refuse(self, t, dtype, name, shape, dense=True):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise TensorLibError(f"{name} must be a CUDA(HIP) tensor; there is no CPU path")
         if t.device.index != self.ordinal:
             raise ValueError(f"{name} is on {t.device}, this device is cuda:{self.ordinal}")
         if t.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-        if shape is not None and (t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape))):
+        if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
             raise ValueError(f"{name} must have shape {tuple('any' if w is None else w for w in shape)}, got {tuple(t.shape)}")
-        raise ValueError(f"{name} must be contiguous")
+        raise ValueError(f"{name} must be contiguous" if dense else f"{name} has unsupported strides {t.stride()}")
+
+    def _arg(self, t, dtype, name, *shape):
+        """Pointer of a contiguous tensor of this device with the given type and shape."""
+        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self.ordinal and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+        return self._refuse(t, dtype, name, shape)
+
+    def _any(self, t, dtype, name, dims):
+        """Pointer of a contiguous tensor of this device with the given type and number of dimensions."""
+        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self.ordinal and t.dim() == dims and t.is_contiguous():
+            return t.data_ptr()
+        return self._refuse(t, dtype, name, (None,) * dims)
 
     def _head_rows(self, t, name, heads=None, dim=None):
         """Pointer and row stride of [rows, heads, dim] halves whose heads lie next to each other (rows may be apart)."""
-        p = self._arg(t, torch.float16, name, (None, heads, dim), dense=False)
-        rows, h, d = t.shape
-        rs, hs, ds = t.stride()
-        if (ds != 1 and d > 1) or (hs != d and h > 1) or (rs < h * d and rows > 1):
-            raise ValueError(f"{name}: the heads of a row must be dense and rows must not overlap, got strides {t.stride()}")
-        return p, rs
+        if isinstance(t, torch.Tensor) and t.dtype is torch.float16 and t.get_device() == self.ordinal and t.dim() == 3:
+            n, h, d = t.shape
+            rs, hs, ds = t.stride()
+            if ((heads is None or h == heads) and (dim is None or d == dim) and (ds == 1 or d <= 1) and (hs == d or h <= 1)
+                    and (rs >= h * d or n <= 1)):
+                return t.data_ptr(), rs
+        return self._refuse(t, torch.float16, name, (None, heads, dim), False)
 
-    def _kv_pages(self, k_pages, v_pages):
-        pk = self._arg(k_pages, torch.float16, "k_pages", (None, None, None, None), dense=False)
-        pv = self._arg(v_pages, torch.float16, "v_pages", tuple(k_pages.shape), dense=False)
-        n, ps, h, d = k_pages.shape
-        st = k_pages.stride()
-        if v_pages.stride() != st or (st[3] != 1 and d > 1):
-            raise ValueError(f"k_pages and v_pages need equal strides and dense heads, got {st} and {v_pages.stride()}")
-        return KvPages(pk, pv, st[0], st[1], st[2], n, ps, h, d)
+    def _kv_pages(self, k, v):
+        if isinstance(k, torch.Tensor) and k.dtype is torch.float16 and k.get_device() == self.ordinal and k.dim() == 4:
+            st = k.stride()
+            if (isinstance(v, torch.Tensor) and v.dtype is torch.float16 and v.get_device() == self.ordinal and v.shape == k.shape
+                    and v.stride() == st and (st[3] == 1 or k.shape[3] <= 1)):
+                return KvPages(k.data_ptr(), v.data_ptr(), *st[:3], *k.shape)
+            return self._refuse(v, torch.float16, "v_pages (strides as k_pages, dense heads)", tuple(k.shape), False)
+        return self._refuse(k, torch.float16, "k_pages", (None,) * 4, False)
 
     def _may_allocate(self):
         """Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current
@@ -551,7 +561,7 @@ class HipDevice:
         n, h, d = x.shape
         if layout not in _ROTARY_LAYOUTS:
             raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
-        pp, pf = self._arg(positions, torch.int32, "positions", (n,)), self._arg(freq, torch.float64, "freq", (None,))
+        pp, pf = self._arg(positions, torch.int32, "positions", n), self._any(freq, torch.float64, "freq", 1)
         self._may_allocate()
         if out is None:
             out = torch.empty((n, h, d), dtype=torch.float16, device=x.device)
@@ -577,13 +587,13 @@ class HipDevice:
             raise ValueError("q, k and v must have the same number of tokens")
         if layout not in _ROTARY_LAYOUTS:
             raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
-        pp, pf = self._arg(positions, torch.int32, "positions", (n,)), self._arg(freq, torch.float64, "freq", (None,))
-        ps = None if seq_ids is None else self._arg(seq_ids, torch.int32, "seq_ids", (n,))
-        pt = self._arg(tables, torch.int32, "tables", (None, None))
+        pp, pf = self._arg(positions, torch.int32, "positions", n), self._any(freq, torch.float64, "freq", 1)
+        ps = None if seq_ids is None else self._arg(seq_ids, torch.int32, "seq_ids", n)
+        pt = self._any(tables, torch.int32, "tables", 2)
         self._may_allocate()
         if q_out is None:
             q_out = torch.empty((n, h, d), dtype=torch.float16, device=q.device)
-        po = self._arg(q_out, torch.float16, "q_out", (n, h, d))
+        po = self._arg(q_out, torch.float16, "q_out", n, h, d)
         check(self.lib.tl_rotary_kv_pages_f16(po, pq, sq, pk, sk, pv, sv, pp, ps, pf, 2 * freq.numel(), _ROTARY_LAYOUTS[layout], magnitude, n, h,
                                               cache, pt, tables.shape[1], tables.shape[0]), "tl_rotary_kv_pages_f16")
         return q_out
@@ -598,18 +608,20 @@ class HipDevice:
         d = cache.head_dim
         pq, sq = self._head_rows(q, "q", None, d)
         b, h, _ = q.shape
-        pt, pl = self._arg(tables, torch.int32, "tables", (b, None)), self._arg(lens, torch.int32, "lens", (b,))
-        width = tables.shape[1]
+        pt, pl = self._any(tables, torch.int32, "tables", 2), self._arg(lens, torch.int32, "lens", b)
+        rows, width = tables.shape
+        if rows != b:
+            raise ValueError(f"tables must have {b} rows, got {rows}")
         if max_len is None:
             max_len = min(width * cache.page_size, 2 ** 31 - 1)
         self._may_allocate()
         if out is None:
             out = torch.empty((b, h, d), dtype=torch.float16, device=q.device)
-        po = self._arg(out, torch.float16, "out", (b, h, d))
+        po = self._arg(out, torch.float16, "out", b, h, d)
         need = self.lib.tl_paged_attention_workspace(b, h, cache.n_kv_heads, d, max_len)
         if workspace is None and need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        pw = None if workspace is None else self._arg(workspace, torch.uint8, "workspace")
+        pw = None if workspace is None else self._any(workspace, torch.uint8, "workspace", 1)
         check(self.lib.tl_paged_attention_f16(po, pq, sq, cache, pt, width, pl, b, h, max_len, 1.0 / math.sqrt(d) if scale is None else scale, pw,
                                               0 if workspace is None else workspace.numel()), "tl_paged_attention_f16")
         return out
@@ -620,13 +632,12 @@ class HipDevice:
 
     @staticmethod
     def _int_arrays(like, *sizes):
-        """int32 arrays of these sizes out of one allocation, each 16-byte aligned."""
-        room = [(n + 3) & ~3 for n in sizes]
-        return [t if t.shape[0] == n else t[:n] for t, n in zip(like.new_empty(sum(room)).split(room), sizes)]
+        """int32 arrays of these sizes out of one allocation."""
+        return like.new_empty(sum(sizes)).split_with_sizes(sizes)
 
     def _page_state(self, tables, lens, refs):
-        pt = self._arg(tables, torch.int32, "tables", (None, None))
-        return pt, self._arg(lens, torch.int32, "lens", (tables.shape[0],)), self._arg(refs, torch.int32, "refs", (None,))
+        pt = self._any(tables, torch.int32, "tables", 2)
+        return pt, self._arg(lens, torch.int32, "lens", tables.shape[0]), self._any(refs, torch.int32, "refs", 1)
 
     def pages_fork(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int):
         """Row i of the new state continues sequence parents[i] (-1: empty). Returns (tables, lens, refs, copy_src, copy_dst,
@@ -634,7 +645,7 @@ class HipDevice:
         free pages, the state is unchanged."""
         pt, pl, pr = self._page_state(tables, lens, refs)
         n, width = tables.shape
-        pp = self._arg(parents, torch.int32, "parents", (n,))
+        pp = self._arg(parents, torch.int32, "parents", n)
         self._may_allocate()
         t, ln, r, src, dst, missing = self._int_arrays(tables, n * width, n, refs.shape[0], n, n, 1)
         t = t.view(n, width)
@@ -646,7 +657,7 @@ class HipDevice:
         """Room for add[i] more positions of every sequence, in place. Returns missing ([1]): 0, or why nothing changed."""
         pt, pl, pr = self._page_state(tables, lens, refs)
         n, width = tables.shape
-        pa = self._arg(add, torch.int32, "add", (n,))
+        pa = self._arg(add, torch.int32, "add", n)
         self._may_allocate()
         missing = tables.new_empty(1)
         check(self.lib.tl_pages_extend(pt, pl, pr, pa, missing.data_ptr(), n, width, refs.shape[0], page_size), "tl_pages_extend")
@@ -656,13 +667,13 @@ class HipDevice:
         """Gives back the pages of the sequences with rows[i] true and empties them, in place."""
         pt, pl, pr = self._page_state(tables, lens, refs)
         n, width = tables.shape
-        pw = self._arg(rows, torch.bool, "rows", (n,))
+        pw = self._arg(rows, torch.bool, "rows", n)
         check(self.lib.tl_pages_free(pt, pl, pr, pw, n, width, refs.shape[0], page_size), "tl_pages_free")
 
     def pages_compact(self, tables: torch.Tensor, refs: torch.Tensor):
         """Moves the live pages to the low end of the pool. Returns (tables, refs, remap, copy_src, copy_dst, count);
         pages_copy(pool, copy_src, copy_dst, count) then moves the data."""
-        pt, pr = self._arg(tables, torch.int32, "tables", (None, None)), self._arg(refs, torch.int32, "refs", (None,))
+        pt, pr = self._any(tables, torch.int32, "tables", 2), self._any(refs, torch.int32, "refs", 1)
         self._may_allocate()
         n, width = tables.shape
         pages = refs.shape[0]
@@ -677,35 +688,43 @@ class HipDevice:
         count[0] on."""
         if not isinstance(pool, torch.Tensor) or pool.dim() < 3:
             raise ValueError("pool must be [planes, pages, ...page]")
-        p = self._arg(pool, pool.dtype, "pool", dense=False)
+        if pool.get_device() != self.ordinal:
+            self._refuse(pool, pool.dtype, "pool", tuple(pool.shape))
+        p = pool.data_ptr()
         item = pool.element_size()
-        planes, pages = pool.shape[:2]
-        if pool.numel() and not pool[0, 0].is_contiguous():
-            raise ValueError("a page of the pool must be contiguous")
-        ps, pd = self._arg(src, torch.int32, "src", (None,)), self._arg(dst, torch.int32, "dst", (src.shape[0],))
-        pc = None if count is None else self._arg(count, torch.int32, "count", (1,))
-        page_bytes = math.prod(pool.shape[2:]) * item
-        check(self.lib.tl_pages_copy(p, pool.stride(0) * item, pool.stride(1) * item, page_bytes, planes, pages, ps, pd, pc, src.shape[0]),
+        planes, pages, *page = pool.shape
+        plane_stride, page_stride, *inner = pool.stride()
+        page_bytes = item
+        for extent, stride in zip(reversed(page), reversed(inner)):
+            if stride * item != page_bytes and extent > 1:
+                raise ValueError("a page of the pool must be contiguous")
+            page_bytes *= extent
+        ps, pd = self._any(src, torch.int32, "src", 1), self._arg(dst, torch.int32, "dst", src.shape[0])
+        pc = None if count is None else self._arg(count, torch.int32, "count", 1)
+        check(self.lib.tl_pages_copy(p, plane_stride * item, page_stride * item, page_bytes, planes, pages, ps, pd, pc, src.shape[0]),
               "tl_pages_copy")
 
     def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, n_beams: int, finished: torch.Tensor | None = None, end_token: int = 2,
                     n_select: int | None = None, workspace: torch.Tensor | None = None):
         """logits [requests * n_beams, vocab] (rows may be apart), scores (float32) and finished (bool) per row. Returns the best
         n_select (default n_beams) continuations of every request as flat (scores, tokens, parents), best first."""
-        pl = self._arg(logits, torch.float16, "logits", (None, None), dense=False)
+        if not (isinstance(logits, torch.Tensor) and logits.dtype is torch.float16 and logits.get_device() == self.ordinal and logits.dim() == 2):
+            self._refuse(logits, torch.float16, "logits", (None, None), False)
+        pl = logits.data_ptr()
         rows, vocab = logits.shape
-        if n_beams < 1 or rows % n_beams or logits.stride(1) != 1 and vocab > 1 or logits.stride(0) < vocab and rows > 1:
+        row_stride, one = logits.stride()
+        if n_beams < 1 or rows % n_beams or one != 1 and vocab > 1 or row_stride < vocab and rows > 1:
             raise ValueError(f"logits must be [requests * {n_beams}, vocab] with dense rows, got {tuple(logits.shape)}, strides {logits.stride()}")
-        ps = self._arg(scores, torch.float32, "scores", (rows,))
-        pf = None if finished is None else self._arg(finished, torch.bool, "finished", (rows,))
+        ps = self._arg(scores, torch.float32, "scores", rows)
+        pf = None if finished is None else self._arg(finished, torch.bool, "finished", rows)
         batch, n = rows // n_beams, n_beams if n_select is None else n_select
         self._may_allocate()
         out = torch.empty(max(batch * n, 0), dtype=torch.float32, device=logits.device)
         tokens, parents = torch.empty_like(out, dtype=torch.int32), torch.empty_like(out, dtype=torch.int32)
         if workspace is None:
             workspace = torch.empty(self.lib.tl_beam_select_workspace(batch, n_beams, vocab, n), dtype=torch.uint8, device=logits.device)
-        pw = self._arg(workspace, torch.uint8, "workspace")
-        check(self.lib.tl_beam_select_f16(out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), pl, logits.stride(0), ps, pf, batch, n_beams, vocab, n,
+        pw = self._any(workspace, torch.uint8, "workspace", 1)
+        check(self.lib.tl_beam_select_f16(out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), pl, row_stride, ps, pf, batch, n_beams, vocab, n,
                                           end_token, pw, workspace.numel()), "tl_beam_select_f16")
         return out, tokens, parents
 
@@ -717,13 +736,13 @@ class HipDevice:
                      tokens: torch.Tensor, end_token: int = 2):
         """The histories [rows, width] after a selection: row i is parents[i]'s with tokens[i] behind it. Returns (history, lens,
         finished)."""
-        ph = self._arg(history, torch.int32, "history", (None, None))
+        ph = self._any(history, torch.int32, "history", 2)
         rows, width = history.shape
-        pl = self._arg(lens, torch.int32, "lens", (rows,))
-        pf = None if finished is None else self._arg(finished, torch.bool, "finished", (rows,))
-        pp = self._arg(parents, torch.int32, "parents", (None,))
+        pl = self._arg(lens, torch.int32, "lens", rows)
+        pf = None if finished is None else self._arg(finished, torch.bool, "finished", rows)
+        pp = self._any(parents, torch.int32, "parents", 1)
         n = parents.shape[0]
-        pt = self._arg(tokens, torch.int32, "tokens", (n,))
+        pt = self._arg(tokens, torch.int32, "tokens", n)
         self._may_allocate()
         h = torch.empty((n, width), dtype=torch.int32, device=history.device)
         ln, f = torch.empty(n, dtype=torch.int32, device=history.device), torch.empty(n, dtype=torch.bool, device=history.device)

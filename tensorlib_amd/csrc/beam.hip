@@ -5,26 +5,33 @@
 // score.  The sum of a row is held in fp64 and scores are compared in fp64: candidates of different beams may lie
 // closer than an fp32 rounding.
 //
-// Bound by the one pass over the logits (2 bytes each; small requests by latency).  First launch: one workgroup per
-// (row, slice of the vocabulary) holds its slice in registers, leaves the slice's maximum and sum and its best n
-// candidates: within a row, the order of the logits is the order of the scores, so no sum is needed for that.  Second
-// launch: one workgroup per request joins the rows' sums and picks.
+// Bound by the one pass over the logits (2 bytes each), small requests by latency.  First launch: one workgroup per (row,
+// slice of the vocabulary) holds its slice in registers and leaves the slice's maximum, its sum and its best n
+// candidates in order: within a row the order of the logits is the order of the scores, so no sum is needed for that.
+// Second launch: one workgroup per request joins the rows' sums and picks.
+//
+// The best n of many, in both launches: cut the lanes into G >= n groups; the smallest of the groups' maxima is a bound that
+// at least n elements reach.  The groups may be those of one wavefront, or a share of each wavefront's; the largest such
+// bound is taken.  What reaches it (some twenty candidates for n = 8 out of 8192 random logits) goes to a list in LDS,
+// where every candidate counts those before it: its rank is its place in the answer.  A list that overflows (values in an order that defeats the bound) is given up
+// for n rounds of a maximum over the workgroup.
 #include <cmath>
 
-#include "tl_internal.h"
+#include "paged.h"
 
 namespace tl {
 
 typedef unsigned long long u64;
 
 constexpr int kBeamThreads = 256;
-constexpr int kPerThread = 32;                            // logits a thread holds
-constexpr int kSlice = kBeamThreads * kPerThread;
+constexpr int kBeamWaves = kBeamThreads / 64;
+constexpr int kIndexBits = 13;                            // of a logit in its slice
 constexpr int kMaxSelect = 64;
+constexpr int kList = 1024;
 
 struct SliceStats {
-    double sum;                                           // of exp(logit - top)
-    float top;
+    double sum;                                           // of 2^(logit log2 e - top), NaN if the slice holds NaN or +inf
+    float top;                                            // largest logit times log2 e, as rounded; -inf: nothing but -inf
     float pad;
 };
 
@@ -36,177 +43,359 @@ struct BeamArgs {
     float* scores_out;
     int *tokens_out, *parents_out;
     SliceStats* stats;                                    // [row][slice]
-    u64* best;                                            // [row][slice][n_select]
-    int n_beams, vocab, n_select, end_token, n_slices;
+    unsigned* best;                                       // [row][slice][n_select]
+    FastDiv by_row;                                       // candidates per row in the second launch
+    int n_beams, vocab, n_select, end_token, n_slices, slice, groups_log2;
 };
 
-// Larger is better: the logit's order (the two zeros are equal), then the lower index.  Never 0.
-__device__ __forceinline__ u64 candidate(half_t x, int index) {
+// Larger is better: the logit's order (the two zeros are equal), then the lower index in the slice.  Never 0.
+__device__ __forceinline__ unsigned key_of(half_t x) {
     unsigned b = __builtin_bit_cast(unsigned short, x);
     if (b == 0x8000u) b = 0;
-    b = b & 0x8000u ? (~b & 0xffffu) : (b | 0x8000u);
-    return ((u64)b << 32) | (unsigned)~index;
+    return b & 0x8000u ? (~b & 0xffffu) : (b | 0x8000u);
 }
-__device__ __forceinline__ float candidate_logit(u64 c) {
-    unsigned b = (unsigned)(c >> 32);
+__device__ __forceinline__ unsigned candidate(half_t x, int index) { return (key_of(x) << kIndexBits) | (unsigned)((1 << kIndexBits) - 1 - index); }
+__device__ __forceinline__ float candidate_logit(unsigned c) {
+    unsigned b = c >> kIndexBits;
     b = b & 0x8000u ? (b & 0x7fffu) : (~b & 0xffffu);
     return (float)__builtin_bit_cast(half_t, (unsigned short)b);
 }
-__device__ __forceinline__ int candidate_index(u64 c) { return (int)~(unsigned)c; }
+__device__ __forceinline__ int candidate_index(unsigned c) { return (1 << kIndexBits) - 1 - (int)(c & ((1u << kIndexBits) - 1)); }
 
-__device__ __forceinline__ u64 wave_max(u64 v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d /= 2) {
-        const u64 o = __shfl_xor(v, d, 64);
-        v = o > v ? o : v;
+// v of the lane with one bit of its number flipped, for values that are equal within groups of 2^BIT adjacent lanes (what the
+// steps of a reduction over lanes leave behind): within 16 lanes by moves in the vector pipe, not through LDS.
+template <int BIT, class T>
+__device__ __forceinline__ T other_half(T v) {
+    if constexpr (BIT >= 4) {
+        return __shfl_xor(v, 1 << BIT, 64);
+    } else {
+        constexpr int ctrl = BIT == 0 ? 0xB1 : BIT == 1 ? 0x4E : BIT == 2 ? 0x141 : 0x140;     // quads, then mirrored halves
+        if constexpr (sizeof(T) == 4) {
+            return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true));
+        } else {
+            const int2 w = __builtin_bit_cast(int2, v);
+            return __builtin_bit_cast(T, int2{__builtin_amdgcn_update_dpp(0, w.x, ctrl, 0xf, 0xf, true), __builtin_amdgcn_update_dpp(0, w.y, ctrl, 0xf, 0xf, true)});
+        }
     }
-    return v;
+}
+template <class T, class F>
+__device__ __forceinline__ T over_wave(T v, F f) {
+    v = f(v, other_half<0>(v), 0);
+    v = f(v, other_half<1>(v), 1);
+    v = f(v, other_half<2>(v), 2);
+    v = f(v, other_half<3>(v), 3);
+    v = f(v, other_half<4>(v), 4);
+    return f(v, other_half<5>(v), 5);
+}
+template <class T>
+__device__ __forceinline__ T wave_max(T v) {
+    return over_wave(v, [](T a, T b, int) { return b > a ? b : a; });
+}
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
+    return over_wave(v, [](T a, T b, int) { return a + b; });
+}
+// The smallest over 2^groups_log2 groups of adjacent lanes of the group's largest value.
+template <class T>
+__device__ __forceinline__ T smallest_group_maximum(T v, int groups_log2) {
+    return over_wave(v, [groups_log2](T a, T b, int bit) { return (bit < 6 - groups_log2) == (b > a) ? b : a; });
 }
 
-// exp(d) for d <= 0 to about an ulp: the product with log2 e is carried in two floats.
-__device__ __forceinline__ float exp_of(float d) {
-    const float hi = d * 1.4426950408889634f;
-    const float lo = __builtin_fmaf(d, 1.4426950408889634f, -hi) + d * 1.9259629911266175e-8f;
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return d == -INFINITY ? 0.f : __builtin_fmaf(e, lo * 0.6931471805599453f, e);
-}
+constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.925963033500011e-8f;      // the sum is log2 e to 2^-49
 
+// NV: 16-byte pieces of logits per thread; a slice is NV * 2048 of them.
+template <int NV>
 __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
-    __shared__ u64 s_best[kBeamThreads / 64];
-    __shared__ float s_top[kBeamThreads / 64];
-    __shared__ double s_sum[kBeamThreads / 64];
-    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    constexpr int SLICE = NV * kBeamThreads * 8;
+    static_assert(SLICE <= 1 << kIndexBits, "index bits");
+    __shared__ __align__(16) unsigned s_list[kList];
+    __shared__ unsigned s_bound[kBeamWaves], s_share[kBeamWaves], s_best[kBeamWaves];
+    __shared__ half_t s_top[kBeamWaves];
+    __shared__ double s_sum[kBeamWaves];
+    __shared__ int s_count;
+    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, wave = tid / 64;
     if (A.finished && A.finished[row]) return;
-    const int v0 = slice * kSlice;
-    const int n = A.vocab - v0 < kSlice ? A.vocab - v0 : kSlice;
+    const int v0 = slice * SLICE;
+    const int n = A.vocab - v0 < SLICE ? A.vocab - v0 : SLICE;
     const half_t* x = A.logits + (size_t)row * A.logits_stride + v0;
-    half_t v[kPerThread];
-    float top = -INFINITY;
-    bool odd = false;                                     // NaN or +inf: the row has no probabilities
+    half8_t v[NV];
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-        const int i = j * kBeamThreads + tid;
-        v[j] = i < n ? x[i] : (half_t)-INFINITY;
-        odd |= !((float)v[j] < INFINITY);
-        top = fmaxf(top, (float)v[j]);
+    for (int j = 0; j < NV; ++j) {
+        const int i = (j * kBeamThreads + tid) * 8;
+        if (i + 8 <= n) {
+            __builtin_memcpy(&v[j], x + i, 16);           // rows of an odd vocabulary start at any even address
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = i + e < n ? x[i + e] : (half_t)-INFINITY;
+        }
     }
+    if (tid == 0) s_count = 0;
+    // the largest logit of each piece and of the thread; NaN shows in the sum
+    half_t most[NV], top = (half_t)-INFINITY;
 #pragma unroll
-    for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-    if (tid % 64 == 0) s_top[tid / 64] = top;
-    odd = __syncthreads_or(odd);
-    for (int w = 0; w < kBeamThreads / 64; ++w) top = fmaxf(top, s_top[w]);
+    for (int j = 0; j < NV; ++j) {
+        half2_t m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = half2_t{v[j][2 * e], v[j][2 * e + 1]};
+        m[0] = __builtin_elementwise_max(__builtin_elementwise_max(m[0], m[1]), __builtin_elementwise_max(m[2], m[3]));
+        most[j] = __builtin_elementwise_max(m[0][0], m[0][1]);
+        top = __builtin_elementwise_max(top, most[j]);
+    }
+    int first = NV - 1;                                   // the first piece that holds it
+#pragma unroll
+    for (int j = NV - 2; j >= 0; --j)
+        if (most[j] == top) first = j;
+    // the candidate of the piece's last element is at most the thread's best: still a bound that enough elements reach
+    const unsigned mine_least = candidate(top, (first * kBeamThreads + tid) * 8 + 7);
+    const unsigned bound = smallest_group_maximum(mine_least, A.groups_log2);
+    const unsigned share = smallest_group_maximum(mine_least, A.groups_log2 > 2 ? A.groups_log2 - 2 : 0);
+    const float wave_top = wave_max((float)top);
+    if (tid % 64 == 0) {
+        s_bound[wave] = bound;
+        s_share[wave] = share;
+        s_top[wave] = (half_t)wave_top;
+    }
+    __syncthreads();
+    unsigned reach = 0, all = ~0u;
+    float slice_top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kBeamWaves; ++w) {
+        reach = max(reach, s_bound[w]);
+        all = min(all, s_share[w]);
+        slice_top = fmaxf(slice_top, (float)s_top[w]);
+    }
+    reach = max(reach, all);
+    // sum of 2^(x log2 e - c) with c as it was rounded: the logarithm gets exactly that c back
+    const float c = slice_top == -INFINITY ? 0.f : slice_top * kLog2eHi;
     double sum = 0.0;
-    if (top > -INFINITY && !odd) {
 #pragma unroll
-        for (int j = 0; j < kPerThread; ++j) sum += (double)exp_of((float)v[j] - top);
+    for (int j = 0; j < NV; ++j) {
+        float part[2] = {0.f, 0.f};                       // four terms each, then fp64
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = (float)v[j][e];
+            part[e % 2] += __builtin_amdgcn_exp2f(__builtin_fmaf(f, kLog2eLo, __builtin_fmaf(f, kLog2eHi, -c)));   // -inf: 0
+        }
+        sum += (double)part[0] + (double)part[1];
     }
+    // what reaches the bound
+    const half_t reach_value = (half_t)candidate_logit(reach);
 #pragma unroll
-    for (int d = 32; d >= 1; d /= 2) sum += __shfl_xor(sum, d, 64);
-    if (tid % 64 == 0) s_sum[tid / 64] = sum;
+    for (int j = 0; j < NV; ++j) {
+        if (!(most[j] >= reach_value)) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (!(v[j][e] >= reach_value)) continue;
+            const int i = (j * kBeamThreads + tid) * 8 + e;
+            const unsigned cand = candidate(v[j][e], i);
+            if (cand >= reach && i < n) {
+                const int at = atomicAdd(&s_count, 1);
+                if (at < kList) s_list[at] = cand;
+            }
+        }
+    }
+    sum = wave_sum(sum);
+    if (tid % 64 == 0) s_sum[wave] = sum;
     __syncthreads();
     if (tid == 0) {
         sum = 0.0;
-        for (int w = 0; w < kBeamThreads / 64; ++w) sum += s_sum[w];
-        A.stats[(size_t)row * A.n_slices + slice] = {odd ? (double)NAN : sum, top, 0.f};
+        for (int w = 0; w < kBeamWaves; ++w) sum += s_sum[w];
+        A.stats[(size_t)row * A.n_slices + slice] = {slice_top < INFINITY ? sum : (double)NAN, slice_top == -INFINITY ? -INFINITY : c, 0.f};
     }
-    u64 bound = ~0ull;                                    // candidates below it have not been taken
-    u64* best = A.best + ((size_t)row * A.n_slices + slice) * A.n_select;
-    for (int k = 0; k < A.n_select; ++k) {
-        u64 mine = 0;
-#pragma unroll
-        for (int j = 0; j < kPerThread; ++j) {
-            const int i = j * kBeamThreads + tid;
-            const u64 c = candidate(v[j], v0 + i);
-            if (i < n && c < bound && c > mine) mine = c;
+    unsigned* best = A.best + ((size_t)row * A.n_slices + slice) * A.n_select;
+    const int count = s_count;
+    if (count <= kList) {
+        for (int i = tid; i < count; i += kBeamThreads) {
+            const unsigned mine = s_list[i];
+            int rank = 0;
+            for (int k = 0; k < count; k += 8) {          // what stands behind the list's end is masked
+                const uint4 a = *reinterpret_cast<const uint4*>(s_list + k), b = *reinterpret_cast<const uint4*>(s_list + k + 4);
+                rank += (a.x > mine) + (k + 1 < count && a.y > mine) + (k + 2 < count && a.z > mine) + (k + 3 < count && a.w > mine);
+                rank += (k + 4 < count && b.x > mine) + (k + 5 < count && b.y > mine) + (k + 6 < count && b.z > mine) + (k + 7 < count && b.w > mine);
+            }
+            if (rank < A.n_select) best[rank] = mine;
         }
+        for (int i = count + tid; i < A.n_select; i += kBeamThreads) best[i] = 0;       // the slice has no more
+        return;
+    }
+    unsigned below = ~0u;
+    for (int k = 0; k < A.n_select; ++k) {
+        unsigned mine = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = (j * kBeamThreads + tid) * 8 + e;
+                const unsigned cand = candidate(v[j][e], i);
+                if (i < n && cand < below && cand > mine) mine = cand;
+            }
         mine = wave_max(mine);
         __syncthreads();
-        if (tid % 64 == 0) s_best[tid / 64] = mine;
+        if (tid % 64 == 0) s_best[wave] = mine;
         __syncthreads();
-        mine = s_best[0];
-        for (int w = 1; w < kBeamThreads / 64; ++w) mine = s_best[w] > mine ? s_best[w] : mine;
-        if (tid == 0) best[k] = mine;                     // 0: the slice has no more
-        bound = mine;
+#pragma unroll
+        for (int w = 0; w < kBeamWaves; ++w) mine = max(mine, s_best[w]);
+        if (tid == 0) best[k] = mine;
+        below = mine;
     }
 }
 
-// A continuation of a request: better by score, then by the lower place beam * vocab + token.
+// A continuation of a request: better by score, then by the lower place.
 struct Choice {
     double score;
-    u64 place;
+    u64 place;                                            // beam, then token
 };
 __device__ __forceinline__ bool better(const Choice& a, const Choice& b) { return a.score > b.score || (a.score == b.score && a.place < b.place); }
 
-__global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(BeamArgs A) {
-    __shared__ Choice s_best[kBeamThreads / 64];
+constexpr int kPickThreads = 1024;
+constexpr int kPickWaves = kPickThreads / 64;
+constexpr int kHeld = 4;                                  // continuations a thread keeps in registers
+
+__global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
+    __shared__ Choice s_list[kList];
+    __shared__ Choice s_best[kPickWaves];
     __shared__ Choice s_last;
-    extern __shared__ double s_base[];                    // per beam: score - log sum, or -inf for a beam without continuations
-    const int request = blockIdx.x, tid = threadIdx.x;
-    for (int b = tid; b < A.n_beams; b += kBeamThreads) {
-        const int row = request * A.n_beams + b;
-        const double score = (double)A.scores[row];
-        double base = -INFINITY;
-        if (A.finished && A.finished[row]) {
-            base = score;
-        } else {
-            const SliceStats* st = A.stats + (size_t)row * A.n_slices;
-            float top = -INFINITY;
-            for (int s = 0; s < A.n_slices; ++s) top = fmaxf(top, st[s].top);
-            double sum = 0.0;
-            for (int s = 0; s < A.n_slices; ++s)
-                sum += st[s].sum == 0.0 ? 0.0 : st[s].sum * exp((double)st[s].top - (double)top);
-            base = score - ((double)top + log(sum));
-        }
-        s_base[b] = base > -INFINITY && base < INFINITY ? base : -INFINITY;
-    }
-    __syncthreads();
+    __shared__ double s_bound[kPickWaves];
+    __shared__ int s_count;
+    extern __shared__ double s_base[];                    // per beam: score - log sum, then how it continues
+    int* s_kind = reinterpret_cast<int*>(s_base + A.n_beams);
+    enum { kDead, kAlive, kFinished };
+    const int request = blockIdx.x, tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    const int row0 = request * A.n_beams;
     const int per_row = A.n_slices * A.n_select;
+    const unsigned total = (unsigned)A.n_beams * A.by_row.d;
     const u64 none = ~0ull;
-    Choice last = {INFINITY, 0};
-    bool first = true;
-    for (int k = 0; k < A.n_select; ++k) {
-        Choice mine = {-INFINITY, none};
-        for (int b = 0; b < A.n_beams; ++b) {
-            const int row = request * A.n_beams + b;
-            const double base = s_base[b];
-            const bool done = A.finished && A.finished[row];
-            const bool dead = !(base > -INFINITY);
-            const int count = done || dead ? A.n_select + 1 : per_row;
-            for (int i = tid; i < count; i += kBeamThreads) {
-                Choice c;
-                if (done || dead) {                       // the end token at the beam's score; all else at -inf, lowest first
-                    if (i >= A.vocab && !(done && i == A.n_select)) continue;
-                    const bool end = done && i == A.n_select;
-                    if (done && !end && i == A.end_token) continue;
-                    c = {end ? base : (double)-INFINITY, (u64)b * A.vocab + (end ? A.end_token : i)};
-                } else {
-                    const u64 e = A.best[(size_t)row * per_row + i];
-                    if (e == 0) continue;
-                    c = {base + (double)candidate_logit(e), (u64)b * A.vocab + candidate_index(e)};
-                }
-                if ((first || better(last, c)) && better(c, mine)) mine = c;
+    // the first candidates are under way while the sums are joined
+    unsigned held[kHeld];
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) {
+        unsigned at = 0, b = 0;
+        const unsigned i = x * kPickThreads + tid;
+        if (i < total) b = A.by_row.divmod(i, at);
+        held[x] = i < total && (int)at < per_row ? A.best[(size_t)(row0 + b) * per_row + at] : 0;
+    }
+    for (int b = wave; b < A.n_beams; b += kPickWaves) {
+        const double score = (double)A.scores[row0 + b];
+        const bool done = A.finished && A.finished[row0 + b];
+        const SliceStats* st = A.stats + (size_t)(row0 + b) * A.n_slices;
+        // a finished row has left nothing there, and nothing of what is read for it is used
+        SliceStats mine = lane < A.n_slices ? st[lane] : SliceStats{0.0, -INFINITY, 0.f};
+        float top = mine.top;
+        for (int s = lane + 64; s < A.n_slices; s += 64) top = fmaxf(top, st[s].top);
+        top = wave_max(top);
+        double sum = 0.0;
+        for (int s = lane;;) {
+            if (mine.sum != 0.0) sum += mine.sum * exp2((double)mine.top - (double)top);
+            s += 64;
+            if (s >= A.n_slices) break;
+            mine = st[s];
+        }
+        sum = wave_sum(sum);
+        const double base = done ? score : score - ((double)top * 0.69314718055994530942 + log(sum));
+        if (lane == 0) {
+            const bool finite = base > -INFINITY && base < INFINITY;
+            s_base[b] = finite ? base : -INFINITY;
+            s_kind[b] = done ? kFinished : finite ? kAlive : kDead;
+        }
+    }
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    // the i-th possible continuation, given its entry of `best`; place none: there is none behind this number
+    auto choice_of = [&](unsigned i, unsigned e) -> Choice {
+        unsigned at;
+        const int b = (int)A.by_row.divmod(i, at);
+        const double base = s_base[b];
+        const int kind = s_kind[b];
+        if (kind != kAlive) {                             // the end token at the beam's score; all else at -inf, lowest first
+            const bool end = kind == kFinished && (int)at == A.n_select;
+            if ((int)at > A.n_select || (!end && ((int)at >= A.vocab || (kind == kFinished && (int)at == A.end_token)))) return {-INFINITY, none};
+            return {end ? base : (double)-INFINITY, (u64)b << 32 | (end ? (unsigned)A.end_token : at)};
+        }
+        if (e == 0) return {-INFINITY, none};
+        return {base + (double)candidate_logit(e), (u64)b << 32 | ((at / A.n_select) * A.slice + candidate_index(e))};
+    };
+    auto choice = [&](unsigned i) -> Choice {
+        unsigned at;
+        const int b = (int)A.by_row.divmod(i, at);
+        return choice_of(i, s_kind[b] == kAlive && (int)at < per_row ? A.best[(size_t)(row0 + b) * per_row + at] : 0);
+    };
+    auto put = [&](int k, const Choice& c) {
+        const size_t o = (size_t)request * A.n_select + k;
+        A.scores_out[o] = (float)c.score;
+        A.tokens_out[o] = (int)(c.place & 0xffffffffu);
+        A.parents_out[o] = row0 + (int)(c.place >> 32);
+    };
+    Choice kept[kHeld];
+    double mine = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) {
+        const unsigned i = x * kPickThreads + tid;
+        kept[x] = {-INFINITY, none};
+        if (i < total) kept[x] = choice_of(i, held[x]);
+        mine = fmax(mine, kept[x].score);
+    }
+    for (unsigned i = kHeld * kPickThreads + tid; i < total; i += kPickThreads) mine = fmax(mine, choice(i).score);
+    const double bound = smallest_group_maximum(mine, A.groups_log2);
+    if (lane == 0) s_bound[wave] = bound;
+    __syncthreads();
+    const double reach = wave_max(s_bound[lane % kPickWaves]);
+    auto list = [&](const Choice& c) {
+        if (c.place == none || !(c.score >= reach)) return;
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kList) s_list[at] = c;
+    };
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) list(kept[x]);
+    for (unsigned i = kHeld * kPickThreads + tid; i < total; i += kPickThreads) list(choice(i));
+    __syncthreads();
+    const int count = s_count;
+    if (count <= kList) {                                 // at least n_select: the bound says so, or everything is in it
+        // P threads count for each choice of the list (a quarter of the threads at least find work)
+        const int parts = count <= kPickThreads / 8 ? 8 : count <= kPickThreads / 4 ? 4 : 1;
+        const int i = tid / parts;
+        if (i < count) {
+            const Choice c = s_list[i];
+            int rank = 0;
+            for (int k = tid % parts; k < count; k += parts) rank += better(s_list[k], c);
+            if (parts >= 4) {
+                rank += other_half<0>(rank);
+                rank += other_half<1>(rank);
             }
+            if (parts == 8) rank += other_half<2>(rank);
+            if (tid % parts == 0 && rank < A.n_select) put(rank, c);
+        }
+        return;
+    }
+    Choice last = {INFINITY, 0};
+    for (int k = 0; k < A.n_select; ++k) {
+        Choice top = {-INFINITY, none};
+        for (unsigned i = tid; i < total; i += kPickThreads) {
+            const Choice c = choice(i);
+            if (c.place != none && (k == 0 || better(last, c)) && better(c, top)) top = c;
         }
 #pragma unroll
         for (int d = 32; d >= 1; d /= 2) {
-            const Choice o = {__shfl_xor(mine.score, d, 64), __shfl_xor(mine.place, d, 64)};
-            if (better(o, mine)) mine = o;
+            const Choice o = {__shfl_xor(top.score, d, 64), __shfl_xor(top.place, d, 64)};
+            if (better(o, top)) top = o;
         }
-        if (tid % 64 == 0) s_best[tid / 64] = mine;
+        if (lane == 0) s_best[wave] = top;
         __syncthreads();
         if (tid == 0) {
-            for (int w = 1; w < kBeamThreads / 64; ++w)
-                if (better(s_best[w], mine)) mine = s_best[w];
-            s_last = mine;
-            const size_t o = (size_t)request * A.n_select + k;
-            A.scores_out[o] = (float)mine.score;
-            A.tokens_out[o] = (int)(mine.place % A.vocab);
-            A.parents_out[o] = request * A.n_beams + (int)(mine.place / A.vocab);
+            for (int w = 1; w < kPickWaves; ++w)
+                if (better(s_best[w], top)) top = s_best[w];
+            s_last = top;
+            put(k, top);
         }
         __syncthreads();
         last = s_last;
-        first = false;
     }
+}
+
+// Vocabulary per workgroup of the first launch: 8192, or 2048 where that leaves compute units without work.
+static int pieces_of(size_t rows, int vocab) { return rows * (((size_t)vocab + 8191) / 8192) >= 256 ? 4 : 1; }
+static size_t slices_of(size_t rows, int vocab) {
+    const size_t slice = (size_t)pieces_of(rows, vocab) * kBeamThreads * 8;
+    return ((size_t)vocab + slice - 1) / slice;
 }
 
 struct AdvanceArgs {
@@ -239,8 +428,8 @@ extern "C" {
 
 size_t tl_beam_select_workspace(int n_batch, int n_beams, int vocab, int n_select) {
     if (n_batch <= 0 || n_beams <= 0 || vocab <= 0 || n_select <= 0) return 0;
-    const size_t slices = ((size_t)vocab + tl::kSlice - 1) / tl::kSlice;
-    return (size_t)n_batch * n_beams * slices * (sizeof(tl::SliceStats) + (size_t)n_select * sizeof(tl::u64));
+    const size_t rows = (size_t)n_batch * n_beams;
+    return rows * tl::slices_of(rows, vocab) * (sizeof(tl::SliceStats) + (size_t)n_select * sizeof(unsigned));
 }
 
 int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, const void* logits, size_t logits_stride, const float* scores,
@@ -257,8 +446,11 @@ int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, con
     TL_REQUIRE((reinterpret_cast<uintptr_t>(logits) & 1u) == 0, "%s: misaligned logits", what);
     TL_REQUIRE(logits_stride >= (size_t)vocab || (n_batch == 1 && n_beams == 1), "%s: the row stride must cover the vocabulary", what);
     const size_t rows = (size_t)n_batch * n_beams;
-    const size_t slices = ((size_t)vocab + kSlice - 1) / kSlice;
     if (rows > 65535) return set_error(TL_ELIMIT, "%s: %zu rows, at most 65535", what, rows);
+    const int pieces = pieces_of(rows, vocab);
+    const size_t slices = slices_of(rows, vocab);
+    const size_t per_row = slices * n_select > (size_t)n_select + 1 ? slices * n_select : (size_t)n_select + 1;
+    if (per_row * n_beams >= (1u << 31)) return set_error(TL_ELIMIT, "%s: a vocabulary of %d is too large for %d beams", what, vocab, n_beams);
     const size_t need = tl_beam_select_workspace(n_batch, n_beams, vocab, n_select);
     TL_REQUIRE(workspace && workspace_bytes >= need && aligned16(workspace), "%s: needs an aligned workspace of %zu bytes, got %zu", what, need,
                workspace ? workspace_bytes : (size_t)0);
@@ -272,15 +464,20 @@ int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, con
     A.tokens_out = tokens_out;
     A.parents_out = parents_out;
     A.stats = static_cast<SliceStats*>(workspace);
-    A.best = reinterpret_cast<u64*>(A.stats + rows * slices);
+    A.best = reinterpret_cast<unsigned*>(A.stats + rows * slices);
+    A.by_row = FastDiv((unsigned)per_row);
     A.n_beams = n_beams;
     A.vocab = vocab;
     A.n_select = n_select;
     A.end_token = end_token;
     A.n_slices = (int)slices;
-    beam_rows_kernel<<<dim3((unsigned)slices, (unsigned)rows), kBeamThreads, 0, stream()>>>(A);
+    A.slice = pieces * kBeamThreads * 8;
+    while ((1 << A.groups_log2) < n_select) ++A.groups_log2;
+    const dim3 grid((unsigned)slices, (unsigned)rows);
+    if (pieces == 4) beam_rows_kernel<4><<<grid, kBeamThreads, 0, stream()>>>(A);
+    else beam_rows_kernel<1><<<grid, kBeamThreads, 0, stream()>>>(A);
     TL_CHECK_LAUNCH("beam_rows_kernel");
-    beam_pick_kernel<<<n_batch, kBeamThreads, n_beams * sizeof(double), stream()>>>(A);
+    beam_pick_kernel<<<n_batch, kPickThreads, n_beams * (sizeof(double) + sizeof(int)), stream()>>>(A);
     TL_CHECK_LAUNCH("beam_pick_kernel");
     return TL_OK;
 }

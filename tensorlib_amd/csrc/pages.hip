@@ -96,33 +96,39 @@ constexpr int kSmallPages = kPer * kThreads;
 constexpr int kSmallSeqs = kThreads;       // a thread per row
 constexpr size_t kSmallEntries = 65536;    // table entries
 
-// The thread's pages [16 tid, 16 tid + 16); pages past the end count as taken.
+// The thread's pages [per tid, per tid + per), per = n_pages / 1024 rounded up; pages past the end count as taken.
 struct MyPages {
-    int ref[kPer];
+    int ref[kPer], per;
+    __device__ __forceinline__ int page(int j) const { return (int)threadIdx.x * per + j; }
     __device__ __forceinline__ void load(const int* refs, int n_pages) {
+        per = (n_pages + kThreads - 1) / kThreads;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const int p = (int)threadIdx.x * kPer + j;
-            ref[j] = p < n_pages ? refs[p] : 1;
+            ref[j] = 1;
+            if (j < per && page(j) < n_pages) ref[j] = refs[page(j)];
         }
     }
-    __device__ __forceinline__ int free_count() const {
+    // How many of the thread's pages fulfil a condition on (page, count).
+    template <class F>
+    __device__ __forceinline__ int count(F f) const {
         int n = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) n += ref[j] == 0;
+        for (int j = 0; j < kPer; ++j)
+            if (j < per) n += f(page(j), ref[j]);
         return n;
     }
-    // Takes those of the thread's free pages whose rank in page order, from `rank` on, is below `wanted`.
+    __device__ __forceinline__ int free_count() const {
+        return count([](int, int r) { return r == 0; });
+    }
+    // Gives away those of the thread's free pages whose rank in page order, from `rank` on, is below `wanted`.
     template <class F>
     __device__ __forceinline__ void take(int rank, int wanted, F give) {
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            if (ref[j] != 0) continue;
-            if (rank < wanted) {
-                ref[j] = 1;
-                give(rank, (int)threadIdx.x * kPer + j);
+            if (j < per && ref[j] == 0) {
+                if (rank < wanted) give(rank, page(j));
+                ++rank;
             }
-            ++rank;
         }
     }
 };
@@ -262,26 +268,19 @@ pages_compact_small_kernel(const int* tables, const int* refs, int* tables_out, 
     const int tid = threadIdx.x;
     MyPages mine;
     mine.load(refs, n_pages);
-    int live = 0, n = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) n += tid * kPer + j < n_pages && mine.ref[j] > 0;
-    block_scan(n, &live);
-    int movers = 0, holes = 0, total;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int p = tid * kPer + j;
-        movers += p < n_pages && p >= live && mine.ref[j] > 0;
-        holes += p < live && mine.ref[j] <= 0;
-    }
-    int m = block_scan(movers, &total), h = block_scan(holes, &holes);
-    movers = total;                        // as many as holes, at most half of the pages
+    int live, total, holes;
+    block_scan(mine.count([&](int p, int ref) { return p < n_pages && ref > 0; }), &live);
+    int m = block_scan(mine.count([&](int p, int ref) { return p < n_pages && p >= live && ref > 0; }), &total);
+    int h = block_scan(mine.count([&](int p, int ref) { return p < live && ref <= 0; }), &holes);
+    const int movers = total;              // as many as holes, at most half of the pages
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        const int p = tid * kPer + j;
-        if (p >= n_pages) break;
-        if (p >= live && mine.ref[j] > 0) s_mover[m++] = (unsigned short)p;
-        if (p < live && mine.ref[j] <= 0) s_hole[h++] = (unsigned short)p;
-        s_new[p] = mine.ref[j] > 0 ? p : -1;
+        const int p = mine.page(j);
+        if (j < mine.per && p < n_pages) {
+            if (p >= live && mine.ref[j] > 0) s_mover[m++] = (unsigned short)p;
+            if (p < live && mine.ref[j] <= 0) s_hole[h++] = (unsigned short)p;
+            s_new[p] = mine.ref[j] > 0 ? p : -1;
+        }
     }
     __syncthreads();
     for (int k = tid; k < movers; k += kThreads) s_new[s_mover[k]] = s_hole[k];

@@ -7,6 +7,7 @@
 // and the rotation itself are fp32, rounded to half once.
 //
 // Bound by memory: every value is read and written once (4 bytes), the positions, frequencies and tables come from L2.
+// 16001 prompt tokens of 32 query and 8 kv heads of 128 take 71 us, 5.5 TB/s; a single token 3.4 us, a launch.
 #include <cmath>
 
 #include "paged.h"
@@ -71,8 +72,9 @@ __device__ __forceinline__ long slot_of(const RotaryArgs& A, size_t token, int p
 
 // One thread: one unit of `ROWS` head rows of a token.  A unit is two 16-byte pieces whose elements pair up (HALF,
 // rotary_dim % 16 == 0), or one piece of four adjacent pairs (rotary_dim % 8 == 0); behind the rotated part, one piece
-// that is copied.  The rows of a thread share their angles, and their loads are in flight together.
-template <bool HALF, int ROWS>
+// that is copied.  The rows of a thread share their angles, and their loads are in flight together.  STREAM: loads and
+// stores that do not settle in the caches.
+template <bool HALF, int ROWS, bool STREAM>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs A) {
     const unsigned id = blockIdx.x * 256u + threadIdx.x;
     if (id >= A.total) return;
@@ -86,6 +88,15 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs A) {
     const int n_rows = A.n_heads + 2 * A.n_kv;
     const long slot = (int)(group * ROWS + ROWS) > A.n_heads ? slot_of(A, token, position) : -1;
 
+    auto load = [](const half_t* p) {
+        const half8_t* v = reinterpret_cast<const half8_t*>(p);
+        return STREAM ? __builtin_nontemporal_load(v) : *v;
+    };
+    auto store = [](half_t* p, half8_t x) {
+        half8_t* v = reinterpret_cast<half8_t*>(p);
+        if (STREAM) __builtin_nontemporal_store(x, v);
+        else *v = x;
+    };
     Row r[ROWS];
     half8_t a[ROWS], b[ROWS];
 #pragma unroll
@@ -93,8 +104,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs A) {
         const int row = (int)group * ROWS + j;
         r[j] = row < n_rows ? row_of(A, token, row, slot) : Row{nullptr, nullptr, false};
         if (r[j].dst) {
-            a[j] = *reinterpret_cast<const half8_t*>(r[j].src + at);
-            if (HALF && turned) b[j] = *reinterpret_cast<const half8_t*>(r[j].src + other);
+            a[j] = load(r[j].src + at);
+            if (HALF && turned) b[j] = load(r[j].src + other);
         }
     }
     float c[8], s[8];
@@ -122,8 +133,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs A) {
                 }
             }
         }
-        *reinterpret_cast<half8_t*>(r[j].dst + at) = a[j];
-        if (HALF && turned) *reinterpret_cast<half8_t*>(r[j].dst + other) = b[j];
+        store(r[j].dst + at, a[j]);
+        if (HALF && turned) store(r[j].dst + other, b[j]);
     }
 }
 
@@ -156,12 +167,18 @@ __global__ void __launch_bounds__(256) rotary_pairs_kernel(RotaryArgs A, int int
     r.dst[i1] = (half_t)y;
 }
 
+// From this many values on, two rows per thread and accesses past the caches (128 dims, 32 + 8 + 8 heads: 512 tokens 5.5 us
+// either way, 1024: 7.3 against 9.2, 16001: 71 against 84 us, 5.5 TB/s); below, one row and plain accesses (64 tokens 3.6
+// against 4.2 us).
+constexpr double kStreamValues = 4194304.0;
+
 static int launch_rotary(RotaryArgs& A, int n_tokens, int layout, bool vectors, const char* what) {
     const bool half = layout == TL_ROTARY_HALF;
     const int n_rows = A.n_heads + 2 * A.n_kv;
     vectors = vectors && A.head_dim % 8 == 0 && A.rotary_dim % (half ? 16 : 8) == 0;
     const int units = vectors ? (half ? A.head_dim / 8 - A.rotary_dim / 16 : A.head_dim / 8) : (A.head_dim + 1) / 2;
-    const int rows = 1;
+    const bool stream_ = vectors && (double)n_tokens * n_rows * A.head_dim >= kStreamValues;
+    const int rows = stream_ ? 2 : 1;
     const int groups = (n_rows + rows - 1) / rows;
     const double total = (double)n_tokens * groups * units;
     if (total >= 2147483648.0) return set_error(TL_ELIMIT, "%s: %d tokens of %d heads of %d are too many for one call", what, n_tokens, n_rows, A.head_dim);
@@ -173,8 +190,10 @@ static int launch_rotary(RotaryArgs& A, int n_tokens, int layout, bool vectors, 
         rotary_pairs_kernel<<<blocks, 256, 0, stream()>>>(A, half ? 0 : 1);
         TL_CHECK_LAUNCH("rotary_pairs_kernel");
     } else {
-        if (half) rotary_kernel<true, 1><<<blocks, 256, 0, stream()>>>(A);
-        else rotary_kernel<false, 1><<<blocks, 256, 0, stream()>>>(A);
+        if (half && stream_) rotary_kernel<true, 2, true><<<blocks, 256, 0, stream()>>>(A);
+        else if (half) rotary_kernel<true, 1, false><<<blocks, 256, 0, stream()>>>(A);
+        else if (stream_) rotary_kernel<false, 2, true><<<blocks, 256, 0, stream()>>>(A);
+        else rotary_kernel<false, 1, false><<<blocks, 256, 0, stream()>>>(A);
         TL_CHECK_LAUNCH("rotary_kernel");
     }
     return TL_OK;

@@ -57,8 +57,9 @@ static size_t attention_lds(int chunk, int group) {
 }
 
 // DP: head_dim rounded up to 64, 128 or 256 (EXACT: equal to it).  U: 16-position tiles per turn of a wavefront; one for
-// DP 256, whose rows fill twice the registers.
-template <int DP, bool EXACT>
+// DP 256, whose rows fill twice the registers.  STREAM: V, whose rows come a whole line per request, is read past the caches (K
+// comes half a line per request, and the second half has to find the first one's line).
+template <int DP, bool EXACT, bool STREAM>
 __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A) {
     constexpr int U = DP == 256 ? 1 : 2;
     constexpr int kTile = 16 * U;         // positions of a turn
@@ -165,8 +166,9 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
                 const half_t* p = vbase + s_slot[s * kTile + 16 * u + 4 * grp + r];
 #pragma unroll
                 for (int x = 0; x < VP; ++x) {
-                    const int d = col * VD + 8 * x;
-                    vf[u][r][x] = *reinterpret_cast<const vpiece*>(p + (EXACT || d < D ? d : 0));
+                    const int d = VP == 1 ? col * VD : 8 * col + 128 * x;      // a row's line is in one request
+                    const vpiece* v = reinterpret_cast<const vpiece*>(p + (EXACT || d < D ? d : 0));
+                    vf[u][r][x] = STREAM ? __builtin_nontemporal_load(v) : *v;
                 }
             }
         asm volatile("" ::: "memory");
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
 #pragma unroll
         for (int i = 0; i < VD; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s_o[(wave * heads + col) * DP + (4 * grp + r) * VD + i] = acc[i][r];
+            for (int r = 0; r < 4; ++r) s_o[(wave * heads + col) * DP + (VP == 1 ? (4 * grp + r) * VD + i : 8 * (4 * grp + r) + 128 * (i / 8) + i % 8)] = acc[i][r];
     }
     __syncthreads();
     const bool whole = len <= A.chunk;    // the only chunk: the result itself
@@ -378,10 +380,11 @@ static int chunk_of(int n_seqs, int head_tiles, int max_len) {
 static int group_tiles_of(int n_heads, int n_kv_heads) { return (n_heads / n_kv_heads + kGroupTile - 1) / kGroupTile; }
 
 template <int DP>
-static void launch_paged_attention(const PagedAttnArgs& A, unsigned blocks) {
+static void launch_paged_attention(const PagedAttnArgs& A, unsigned blocks, bool past) {
     const size_t lds = attention_lds<DP>(A.chunk, A.group);
-    if (A.cache.head_dim == DP) paged_attention_kernel<DP, true><<<blocks, 256, lds, stream()>>>(A);
-    else paged_attention_kernel<DP, false><<<blocks, 256, lds, stream()>>>(A);
+    auto kernel = A.cache.head_dim == DP ? (past ? paged_attention_kernel<DP, true, true> : paged_attention_kernel<DP, true, false>)
+                                         : (past ? paged_attention_kernel<DP, false, true> : paged_attention_kernel<DP, false, false>);
+    kernel<<<blocks, 256, lds, stream()>>>(A);
 }
 
 }  // namespace tl
@@ -439,9 +442,12 @@ int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_k
     A.n_heads = n_heads;
     A.max_len = max_len;
     A.scale_log2 = scale * kLog2e;
-    if (cache->head_dim <= 64) launch_paged_attention<64>(A, (unsigned)blocks);
-    else if (cache->head_dim <= 128) launch_paged_attention<128>(A, (unsigned)blocks);
-    else launch_paged_attention<256>(A, (unsigned)blocks);
+    // V past the caches if what the sequences may read is more than the 256 MB of the last-level one and one pass reads it
+    // (4 x 131072: 320 against 352 us, 64 ragged sequences 115 against 121; a cache of 66 MB that had stayed there 24 against 21)
+    const bool past = A.group_tiles == 1 && (double)n_seqs * max_len * cache->n_kv_heads * cache->head_dim * 4.0 >= 268435456.0;
+    if (cache->head_dim <= 64) launch_paged_attention<64>(A, (unsigned)blocks, past);
+    else if (cache->head_dim <= 128) launch_paged_attention<128>(A, (unsigned)blocks, past);
+    else launch_paged_attention<256>(A, (unsigned)blocks, past);
     TL_CHECK_LAUNCH("paged_attention_kernel");
     if (A.n_splits > 1) {
         // 256 threads where they cover the chunks in one round trip (16 x 8000 positions of 64 dims: 22 us, 24 with 1024),

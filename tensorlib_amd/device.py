@@ -614,6 +614,8 @@ class HipDevice:
             raise ValueError(f"tables must have {b} rows, got {rows}")
         if max_len is None:
             max_len = min(width * cache.page_size, 2 ** 31 - 1)
+        elif not 0 <= max_len < 2 ** 31:
+            raise ValueError(f"max_len {max_len} is out of range")
         self._may_allocate()
         if out is None:
             out = torch.empty((b, h, d), dtype=torch.float16, device=q.device)

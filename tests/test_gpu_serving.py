@@ -59,7 +59,7 @@ def rotated(x, positions, freq, layout, magnitude):
 
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("n,h,d,rd", [(1, 32, 128, 128), (3, 1, 64, 32), (257, 3, 128, 128), (65, 5, 80, 20), (33, 2, 256, 64), (7, 4, 96, 96), (5, 3, 2, 2),
-                                      (9, 2, 7, 4), (4, 2, 33, 32), (6, 3, 64, 0), (1000, 8, 64, 64), (2, 7, 40, 8)])
+                                      (9, 2, 7, 4), (4, 2, 33, 32), (6, 3, 64, 0), (1000, 8, 64, 64), (2, 7, 40, 8), (4101, 9, 128, 64)])
 def test_rotary(dev, layout, n, h, d, rd):
     x = rand((n, h, d), 1)
     rng = np.random.RandomState(n)
@@ -356,7 +356,7 @@ def state(rows, page, width, seed, spare, lens=None):
     return tables, lens, refs, rng
 
 
-@pytest.mark.parametrize("rows,page,width,spare", [(1, 16, 4, 2), (4, 16, 8, 8), (7, 5, 3, 20), (64, 16, 40, 70), (300, 8, 9, 400), (3, 1, 50, 9), (130, 16, 300, 5000)])
+@pytest.mark.parametrize("rows,page,width,spare", [(1, 16, 4, 2), (4, 16, 8, 8), (7, 5, 3, 20), (64, 16, 40, 70), (300, 8, 9, 400), (1100, 8, 5, 1500), (3, 1, 50, 9), (130, 16, 300, 5000)])
 def test_fork_and_extend(dev, rows, page, width, spare):
     tables, lens, refs, rng = state(rows, page, width, rows, spare)
     parents = rng.randint(0, rows, rows)
@@ -465,7 +465,7 @@ def test_compact(dev, n_pages, live):
     assert torch.equal(pool, want) and torch.equal(both, want)
 
 
-@pytest.mark.parametrize("shape", [(1, 5, 8), (4, 300, 16, 2, 64), (3, 20, 16, 8, 128), (2, 9, 24, 3, 72), (64, 7, 8, 1, 8)])
+@pytest.mark.parametrize("shape", [(1, 5, 8), (4, 300, 16, 2, 64), (3, 20, 16, 8, 128), (2, 9, 24, 3, 72), (64, 7, 8, 1, 8), (8, 300, 16, 16, 120)])
 def test_pages_copy(dev, shape):
     pool = rand(shape, 3)
     wide = torch.full((shape[0], shape[1] + 2, math.prod(shape[2:]) + 16), 5.0, dtype=torch.float16, device="cuda")     # pages apart
@@ -547,6 +547,15 @@ def test_beam_select_ties_go_to_the_lowest_index(dev):
     rising = torch.linspace(-40, 40, vocab, device="cuda").half().repeat(rows, 1)       # every thread's last is its best
     check_select(dev, rising, scores, None, beams, 2, 64)
     check_select(dev, rising.flip(1).contiguous(), scores, None, beams, 2, 64)
+    # a dozen low values in the right places leave a bound that thousands of logits reach
+    for n in (8, 64):
+        low = rand((rows, vocab), 6).abs()
+        low.view(rows, -1, 8)[:, torch.arange(vocab // 8, device="cuda") % 64 < 8] -= 20
+        check_select(dev, low, scores, None, beams, 2, n)
+    # all beams alike, each of them with all of the answer
+    same = rand((1, 5000), 7).repeat(64, 1)
+    check_select(dev, same, torch.full((64,), -1.0, device="cuda"), None, 64, 2, 64)
+    check_select(dev, same, -torch.arange(64, device="cuda").float() / 1024, None, 64, 2, 64)
     # a first step: all beams alike, and only the first one counts
     start = torch.tensor([0.0, -math.inf, -math.inf, -math.inf] * 2, device="cuda")
     check_select(dev, rand((1, vocab), 5).repeat(rows, 1), start, None, beams, 2, 4)

@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
             s_slot[x * 64 + lane] = (long)((size_t)page[x] * A.cache.page_stride + (size_t)row[x] * A.cache.row_stride);
     }
     bad = __any(bad);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // other lanes read these offsets
 #pragma unroll
     for (int j = 0; j < KJ; ++j)
         if (col >= heads || (!EXACT && 32 * j + 8 * grp >= D)) qf[j] = zero8;

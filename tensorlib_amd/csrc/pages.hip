@@ -143,7 +143,7 @@ struct ForkArgs {
 // VEC: table entries a thread moves at a time, 4 where rows are 16-byte aligned.
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) {
-    __shared__ int s_len[kSmallSeqs], s_parent[kSmallSeqs], s_first[kSmallSeqs], s_page[kSmallSeqs];
+    __shared__ int s_len[kSmallSeqs], s_pages[kSmallSeqs], s_parent[kSmallSeqs], s_first[kSmallSeqs], s_page[kSmallSeqs];
     extern __shared__ int s_refs[];
     const int r = threadIdx.x;
     const bool row = r < A.n_seqs;
@@ -152,11 +152,12 @@ __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) 
     for (int p = r; p < A.n_pages; p += kThreads) s_refs[p] = A.refs[p];
     s_first[r] = kSmallSeqs;
     s_len[r] = old_len > 0 ? old_len : 0;
+    s_pages[r] = pages_of(old_len, A.page_size, A.table_stride);     // once: the divisions would be half of the loop below
     s_parent[r] = parent >= 0 && parent < A.n_seqs ? parent : -1;
     __syncthreads();
     const bool has = s_parent[r] >= 0;
     const int len = has ? s_len[parent] : 0;
-    const int new_pages = pages_of(len, A.page_size, A.table_stride);
+    const int new_pages = has ? s_pages[parent] : 0;
     const bool partial = len % A.page_size != 0;
     int last = -1;                         // the page to be copied, if the row is not its parent's first
     if (partial) {
@@ -174,8 +175,8 @@ __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) 
         const unsigned to = A.by_vectors.divmod(i, c);
         c *= VEC;
         const int from = s_parent[to];
-        const int old_pages = pages_of(s_len[to], A.page_size, A.table_stride);
-        const int pages = from >= 0 ? pages_of(s_len[from], A.page_size, A.table_stride) : 0;
+        const int old_pages = s_pages[to];
+        const int pages = from >= 0 ? s_pages[from] : 0;
         const int kept = s_page[to] == -2 ? pages - 1 : pages;
         int o[VEC], x[VEC];
 #pragma unroll

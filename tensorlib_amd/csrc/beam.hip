@@ -10,11 +10,14 @@
 // candidates in order: within a row the order of the logits is the order of the scores, so no sum is needed for that.
 // Second launch: one workgroup per request joins the rows' sums and picks.
 //
-// The best n of many, in both launches: cut the lanes into G >= n groups; the smallest of the groups' maxima is a bound that
-// at least n elements reach.  The groups may be those of one wavefront, or a share of each wavefront's; the largest such
-// bound is taken.  What reaches it (some twenty candidates for n = 8 out of 8192 random logits) goes to a list in LDS,
-// where every candidate counts those before it: its rank is its place in the answer.  A list that overflows (values in an order that defeats the bound) is given up
-// for n rounds of a maximum over the workgroup.
+// The best n of many: cut the lanes into G >= n groups; the smallest of the groups' maxima is a bound that at least n elements
+// reach.  The groups may be those of one wavefront, or a share of each wavefront's; the largest such bound is taken.  What reaches it (some twenty candidates for n = 8 out of 8192 random logits) goes to a list in LDS,
+// where every candidate counts those before it: its rank is its place in the answer.  A list that overflows (values in
+// an order that defeats the bound) is given up for n rounds of a maximum over the workgroup.
+//
+// 24 requests of 8 beams over 100003 tokens: 17 + 6 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
+// for 8 us of the first launch, and its workgroups do not all run at a time).  1 request of 4 beams over 32000: 5 + 4 us,
+// two launches and their memory latencies.
 #include <cmath>
 
 #include "paged.h"
@@ -100,6 +103,23 @@ template <class T>
 __device__ __forceinline__ T smallest_group_maximum(T v, int groups_log2) {
     return over_wave(v, [groups_log2](T a, T b, int bit) { return (bit < 6 - groups_log2) == (b > a) ? b : a; });
 }
+
+// The n-th largest of the wavefront's keys, bit by bit from the top.
+__device__ __forceinline__ unsigned nth_largest(unsigned key, int n) {
+    unsigned found = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned trial = found | (1u << bit);
+        if ((int)__popcll(__ballot(key >= trial)) >= n) found = trial;
+    }
+    return found;
+}
+// A float's place in the order of floats, and back.
+__device__ __forceinline__ unsigned order_of(float f) {
+    const unsigned b = __builtin_bit_cast(unsigned, f);
+    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float from_order(unsigned o) { return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu)); }
 
 constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.925963033500011e-8f;      // the sum is log2 e to 2^-49
 
@@ -255,7 +275,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
     __shared__ Choice s_list[kList];
     __shared__ Choice s_best[kPickWaves];
     __shared__ Choice s_last;
-    __shared__ double s_bound[kPickWaves];
+    __shared__ unsigned s_bound[kPickWaves];
     __shared__ int s_count;
     extern __shared__ double s_base[];                    // per beam: score - log sum, then how it continues
     int* s_kind = reinterpret_cast<int*>(s_base + A.n_beams);
@@ -335,10 +355,14 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
         mine = fmax(mine, kept[x].score);
     }
     for (unsigned i = kHeld * kPickThreads + tid; i < total; i += kPickThreads) mine = fmax(mine, choice(i).score);
-    const double bound = smallest_group_maximum(mine, A.groups_log2);
+    // the n-th largest of a wavefront's threads, as a float that is not above it: scores of one beam in neighbouring threads
+    // are in order already, and groups of them would make a loose bound
+    float low = (float)mine;
+    if ((double)low > mine) low = from_order(order_of(low) - 1);
+    const unsigned bound = nth_largest(order_of(low), A.n_select);
     if (lane == 0) s_bound[wave] = bound;
     __syncthreads();
-    const double reach = wave_max(s_bound[lane % kPickWaves]);
+    const double reach = (double)from_order(wave_max(s_bound[lane % kPickWaves]));
     auto list = [&](const Choice& c) {
         if (c.place == none || !(c.score >= reach)) return;
         const int at = atomicAdd(&s_count, 1);
@@ -391,7 +415,8 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
     }
 }
 
-// Vocabulary per workgroup of the first launch: 8192, or 2048 where that leaves compute units without work.
+// Vocabulary per workgroup of the first launch: 8192, or 2048 where that leaves compute units without work (4 rows of 32000:
+// 4.9 us, 5.8 with 8192; 192 rows of 100003: 17 us with 8192, 23 with 2048).
 static int pieces_of(size_t rows, int vocab) { return rows * (((size_t)vocab + 8191) / 8192) >= 256 ? 4 : 1; }
 static size_t slices_of(size_t rows, int vocab) {
     const size_t slice = (size_t)pieces_of(rows, vocab) * kBeamThreads * 8;

@@ -520,7 +520,7 @@ def check_select(dev, logits, scores, finished, n_beams, end, n):
 
 
 @pytest.mark.parametrize("batch,beams,vocab,n", [(1, 1, 1, 1), (1, 4, 32000, 4), (3, 5, 32000, 10), (2, 1, 50, 50), (2, 3, 7, 21), (1, 2, 8192, 64), (5, 8, 8193, 8), (2, 4, 100003, 16),
-                                                 (24, 8, 1000, 8), (1, 40, 300, 40), (7, 3, 16385, 6), (2, 64, 257, 64), (1, 3, 2047, 3)])
+                                                 (24, 8, 1000, 8), (22, 8, 100001, 8), (1, 40, 300, 40), (7, 3, 16385, 6), (2, 64, 257, 64), (1, 3, 2047, 3)])
 def test_beam_select(dev, batch, beams, vocab, n):
     rows = batch * beams
     logits = rand((rows, vocab), 1, 2.5)

@@ -425,7 +425,7 @@ int tl_rotary_f16(void* out, size_t out_stride, const void* in, size_t in_stride
  * rows, in one launch: token t goes to position positions[t] of sequence seq_ids[t] (NULL: sequence t).  q, k, v rows may
  * be column blocks of one projection.  A token whose sequence is not in [0, n_seqs), whose position is negative or past
  * the table, or whose page is not in [0, n_pages) is not stored (its q is still rotated): seq_ids of -1 pad a batch.
- * Two tokens of one call must not have the same cache row. */
+ * Two tokens of one call must not have the same cache row.  q_out may be q if q is dense. */
 int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v, size_t v_stride,
                            const int* positions, const int* seq_ids, const double* freq, int rotary_dim, int layout, float magnitude,
                            int n_tokens, int n_heads, const tl_kv_pages* cache, const int* tables, size_t table_stride, int n_seqs);
@@ -436,7 +436,7 @@ int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const vo
  * launch and the workspace (tl_paged_attention_workspace bytes, 0 if it needs none; nothing in it has to be cleared or
  * survives the call).  lens[b] <= 0 gives zeros; lens[b] beyond max_len or the table, or a page out of range among the
  * pages it covers, gives NaN for that sequence.  Scores, weights and sums are fp32, one rounding at the end.
- * At most 65535 sequences. */
+ * At most 65535 sequences.  out may be q if q is dense. */
 size_t tl_paged_attention_workspace(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len);
 int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_kv_pages* cache, const int* tables, size_t table_stride,
                            const int* lens, int n_seqs, int n_heads, int max_len, float scale, void* workspace, size_t workspace_bytes);

@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
     }
     const int len = A.lens[seq];
     // a length beyond what the tables or the caller's bound cover: the first chunk answers NaN for the sequence
-    const bool too_long = len > A.max_len || (size_t)(len > 0 ? A.by_page.div((unsigned)len - 1u) : 0u) >= A.table_stride;
+    const bool too_long = len > 0 && (len > A.max_len || (size_t)A.by_page.div((unsigned)len - 1u) >= A.table_stride);
     if (split != 0 && (too_long || t0 >= len)) return;
     if (len <= 0 || too_long) {           // nothing to attend to: zeros
         const half_t fill = too_long ? (half_t)NAN : (half_t)0.f;

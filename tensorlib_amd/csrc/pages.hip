@@ -545,7 +545,7 @@ int tl_pages_fork(const int* tables, const int* lens, const int* refs, const int
     if (rc != TL_OK) return rc;
     TL_REQUIRE(refs && refs_out && missing, "%s: null pointer", what);
     TL_REQUIRE(n_seqs == 0 || (tables && lens && parents && tables_out && lens_out && copy_src && copy_dst), "%s: null pointer", what);
-    TL_REQUIRE(tables_out != tables && lens_out != lens && refs_out != refs, "%s: the new state must not lie over the old one", what);
+    TL_REQUIRE((n_seqs == 0 || (tables_out != tables && lens_out != lens)) && refs_out != refs, "%s: the new state must not lie over the old one", what);
     TL_ENSURE_INIT();
     ForkArgs A{tables, lens, refs, parents, tables_out, lens_out, refs_out, copy_src, copy_dst, missing, n_seqs, table_stride, n_pages, page_size, {}};
     if (small_state(n_seqs, table_stride, n_pages)) {

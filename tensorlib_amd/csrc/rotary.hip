@@ -280,7 +280,7 @@ int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const vo
     if (rc != TL_OK) return rc;
     if (n_tokens == 0) return TL_OK;
     TL_REQUIRE(n_seqs >= 0, "%s: negative size", what);
-    TL_REQUIRE(k && v && tables, "%s: null pointer", what);
+    TL_REQUIRE(k && v && (tables || n_seqs == 0 || table_stride == 0), "%s: null pointer", what);
     TL_REQUIRE(n_heads == 0 || (q && q_out), "%s: null pointer", what);
     const size_t D = (size_t)cache->head_dim;
     if (n_tokens > 1)

@@ -737,6 +737,41 @@ def test_a_captured_decode_step_follows_its_inputs(dev):
             assert all(torch.equal(a, c) for a, c in zip(got, want)) and torch.equal(kg, kp) and torch.equal(vg, vp)
 
 
+def test_nothing_to_do(dev):
+    """Empty batches, tables and pools are no error and touch nothing."""
+    none, refs = torch.empty((0, 4), dtype=torch.int32, device="cuda"), ints([1, 0, 2])
+    t, ln, r, src, dst, missing = dev.pages_fork(none, ints([]), refs, ints([]), 8)
+    assert t.shape == (0, 4) and torch.equal(r, refs) and int(missing) == 0 and src.numel() == dst.numel() == 0
+    assert int(dev.pages_extend(none, ints([]), refs, ints([]), 8)) == 0 and r.cpu().tolist() == [1, 0, 2]
+    dev.pages_free(none, ints([]), refs, torch.empty(0, dtype=torch.bool, device="cuda"), 8)
+    t, r, remap, src, dst, count = dev.pages_compact(none, refs)
+    assert r.cpu().tolist() == [1, 2, 0] and remap.cpu().tolist() == [0, -1, 1] and int(count) == 1
+    kp, vp = paged_cache(2, 8, 1, 64, "row")
+    q = rand((3, 2, 64), 1)
+    assert dev.paged_attention(q[:0], kp, vp, none, ints([])).shape == (0, 2, 64)
+    # sequences without any table: nothing to attend to, or a length that no table covers
+    got = dev.paged_attention(q, kp, vp, torch.empty((3, 0), dtype=torch.int32, device="cuda"), ints([0, 0, 1]))
+    assert bool((got[:2] == 0).all()) and torch.isnan(got[2]).all()
+    k0 = kp.clone()
+    dev.rotary_paged(q[:0], q[:0, :1], q[:0, :1], ints([]), None, dev.rotary_frequencies(64), kp, vp, none)
+    dev.rotary_paged(q, q[:, :1], q[:, :1], ints([0, 1, 2]), None, dev.rotary_frequencies(64), kp, vp, none)     # no sequence for any token
+    assert torch.equal(kp, k0)
+    assert all(x.numel() == 0 for x in dev.beam_select(rand((0, 10), 1), torch.empty(0, device="cuda"), 2))
+    h, ln, f = dev.beam_advance(ints([[5, 6]]), ints([2]), None, ints([]), ints([]))
+    assert h.shape == (0, 2) and ln.numel() == f.numel() == 0
+
+
+def test_results_over_their_inputs(dev):
+    """Where input and result may be the same tensor."""
+    kp, vp = paged_cache(12, 8, 2, 64, "row")
+    q, tables, lens = rand((3, 8, 64), 1), ints([[0, 1, 2], [3, 4, 5], [6, 7, 8]]), ints([20, 1, 9])
+    want = dev.paged_attention(q, kp, vp, tables, lens)
+    assert torch.equal(dev.paged_attention(q, kp, vp, tables, lens, out=q), want) and torch.equal(q, want)
+    q, k, freq = rand((3, 8, 64), 1), rand((3, 2, 64), 2), dev.rotary_frequencies(64)
+    want = dev.rotary_paged(q, k, k, lens, None, freq, kp, vp, tables)
+    assert torch.equal(dev.rotary_paged(q, k, k, lens, None, freq, kp, vp, tables, q_out=q), want)
+
+
 def test_front_end_refusals(dev):
     kv, d, page = 2, 64, 16
     kp, vp = paged_cache(4, page, kv, d, "row")

@@ -13,6 +13,7 @@ namespace tl {
 
 constexpr int kThreads = 1024;
 constexpr int kMaxSeqs = 8192;             // the rows' prefix sums sit in LDS
+constexpr int kMaxPages = 1 << 30;         // page numbers are stepped through in int
 
 __device__ __forceinline__ int pages_of(int len, int page_size, int table_stride) {
     if (len <= 0) return 0;
@@ -44,94 +45,76 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
     return before + x - v;
 }
 
-// The number of free pages, counted up to `enough` at least if there are as many (one workgroup).
-__device__ int count_free(const int* refs, int n_pages, int enough) {
-    int found = 0;
-    for (int p0 = 0; p0 < n_pages && found < enough; p0 += 4 * kThreads) {
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int p = p0 + (int)threadIdx.x * 4 + j;
-            if (p < n_pages && refs[p] == 0) ++mine;
-        }
-        int total;
-        block_scan(mine, &total);
-        found += total;
+// A workgroup of 1024 over the reference counts of any number of pages: each wavefront has a sixteenth of them to itself and
+// goes through it in page order, 256 at a time, so that ranks come from ballots and the wavefronts meet only once.
+constexpr int kWaves = kThreads / 64;
+struct PageRange {
+    const int* refs;
+    int n_pages, begin, end;
+    __device__ PageRange(const int* refs_, int n_pages_) : refs(refs_), n_pages(n_pages_) {
+        const long steps = ((long)n_pages + kWaves * 256 - 1) / (kWaves * 256), wave = threadIdx.x / 64;
+        const long b = wave * steps * 256, e = b + steps * 256;
+        begin = b < n_pages ? (int)b : n_pages;
+        end = e < n_pages ? (int)e : n_pages;
     }
-    return found;
-}
-
-// Calls take(k, page) for the `wanted` lowest free pages, k counting from 0 in page order (one workgroup).
-template <class F>
-__device__ void take_free(int* refs, int n_pages, int wanted, F take) {
-    int found = 0;
-    for (int p0 = 0; p0 < n_pages && found < wanted; p0 += 4 * kThreads) {
-        const int p = p0 + (int)threadIdx.x * 4;
-        bool free_[4];
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            free_[j] = p + j < n_pages && refs[p + j] == 0;
-            mine += free_[j];
+    // Four counts of the lane; what lies behind the last page counts as 1, taken and not live: f() never sees it.
+    __device__ __forceinline__ int4 load(int p) const {
+        int4 r = {0, 0, 0, 0};
+        if (p + 4 <= end) __builtin_memcpy(&r, refs + p, 16);
+        else {
+            if (p < end) r.x = refs[p];
+            if (p + 1 < end) r.y = refs[p + 1];
+            if (p + 2 < end) r.z = refs[p + 2];
         }
-        int total;
-        int k = found + block_scan(mine, &total);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!free_[j]) continue;
-            if (k < wanted) {
-                refs[p + j] = 1;
-                take(k, p + j);
-            }
-            ++k;
-        }
-        found += total;
+        return r;
     }
-}
-
-// ---- states that fit one workgroup: the whole operation in one launch, the reference counts in registers or LDS ----
-
-constexpr int kPer = 16;                   // pages per thread
-constexpr int kSmallPages = kPer * kThreads;
-constexpr int kSmallSeqs = kThreads;       // a thread per row
-constexpr size_t kSmallEntries = 65536;    // table entries
-
-// The thread's pages [per tid, per tid + per), per = n_pages / 1024 rounded up; pages past the end count as taken.
-struct MyPages {
-    int ref[kPer], per;
-    __device__ __forceinline__ int page(int j) const { return (int)threadIdx.x * per + j; }
-    __device__ __forceinline__ void load(const int* refs, int n_pages) {
-        per = (n_pages + kThreads - 1) / kThreads;
+    // take(rank, page, count) for the pages of the wavefront's range that f(page, count) picks, ranks from `rank` on; returns
+    // the rank behind the last one.  Stops at a rank of `most`.
+    template <class F, class T>
+    __device__ __forceinline__ int visit(int rank, int most, F f, T take) const {
+        const int lane = threadIdx.x % 64;
+        const unsigned long long below = (1ull << lane) - 1;
+        int4 next = load(begin + lane * 4);
+        for (int p0 = begin; p0 < end && rank < most; p0 += 256) {
+            const int p = p0 + lane * 4;
+            const int4 r = next;
+            if (p0 + 256 < end) next = load(p + 256);
+            const bool pick[4] = {p < end && f(p, r.x), p + 1 < end && f(p + 1, r.y), p + 2 < end && f(p + 2, r.z), p + 3 < end && f(p + 3, r.w)};
+            const unsigned long long b[4] = {__ballot(pick[0]), __ballot(pick[1]), __ballot(pick[2]), __ballot(pick[3])};
+            int mine = rank + (int)(__popcll(b[0] & below) + __popcll(b[1] & below) + __popcll(b[2] & below) + __popcll(b[3] & below));
+            const int count[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            ref[j] = 1;
-            if (j < per && page(j) < n_pages) ref[j] = refs[page(j)];
+            for (int j = 0; j < 4; ++j)
+                if (pick[j]) {
+                    take(mine, p + j, count[j]);
+                    ++mine;
+                }
+            rank += (int)(__popcll(b[0]) + __popcll(b[1]) + __popcll(b[2]) + __popcll(b[3]));
         }
+        return rank;
     }
-    // How many of the thread's pages fulfil a condition on (page, count).
+    // How many pages f picks in the whole pool; *before: in the ranges of the wavefronts before this one.
     template <class F>
-    __device__ __forceinline__ int count(F f) const {
-        int n = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-            if (j < per) n += f(page(j), ref[j]);
-        return n;
-    }
-    __device__ __forceinline__ int free_count() const {
-        return count([](int, int r) { return r == 0; });
-    }
-    // Gives away those of the thread's free pages whose rank in page order, from `rank` on, is below `wanted`.
-    template <class F>
-    __device__ __forceinline__ void take(int rank, int wanted, F give) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            if (j < per && ref[j] == 0) {
-                if (rank < wanted) give(rank, page(j));
-                ++rank;
-            }
+    __device__ int count(F f, int* before) const {
+        __shared__ int s_count[kWaves];
+        const int n = visit(0, 0x7fffffff, f, [](int, int, int) {});
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) s_count[threadIdx.x / 64] = n;
+        __syncthreads();
+        int all = 0;
+        *before = 0;
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < (int)threadIdx.x / 64) *before += s_count[w];
+            all += s_count[w];
         }
+        return all;
     }
 };
+__device__ __forceinline__ bool is_free(int, int count) { return count == 0; }
+
+constexpr int kSmallPages = 16384;         // a fork of at most this in one launch: the counts fit LDS,
+constexpr int kSmallSeqs = kThreads;       // the rows a thread each,
+constexpr size_t kSmallEntries = 32768;    // and the tables' entries are soon gone through
 
 struct ForkArgs {
     const int *tables, *lens, *refs, *parents;
@@ -140,7 +123,9 @@ struct ForkArgs {
     FastDiv by_vectors;                    // table entries of a row, in steps of VEC
 };
 
-// VEC: table entries a thread moves at a time, 4 where rows are 16-byte aligned.
+// A fork in one launch, one workgroup (48 x 4 rows of 128 entries 10 us, against 13 for the three launches below and two more
+// from the host; at 65536 entries 23 against 18).  VEC: table entries a thread moves at a time, 4 where rows are 16-byte
+// aligned.
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) {
     __shared__ int s_len[kSmallSeqs], s_pages[kSmallSeqs], s_parent[kSmallSeqs], s_first[kSmallSeqs], s_page[kSmallSeqs];
@@ -205,13 +190,13 @@ __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) 
     }
     __syncthreads();
     const bool wants = copied && last >= 0 && last < A.n_pages;
-    int wanted, available;
+    int wanted, before = 0;
     const int rank = block_scan(wants, &wanted);
-    MyPages mine;
-    mine.load(s_refs, A.n_pages);
-    const int before = block_scan(mine.free_count(), &available);
+    const PageRange range(s_refs, A.n_pages);
+    const int available = wanted ? range.count(is_free, &before) : 0;
     const bool enough = available >= wanted;
-    if (enough) mine.take(before, wanted, [&](int k, int page) {
+    if (enough) range.visit(before, wanted, is_free, [&](int k, int page, int) {
+        if (k >= wanted) return;
         s_page[k] = page;
         s_refs[page] = 1;
     });
@@ -228,80 +213,6 @@ __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) 
     if (!enough)
         for (size_t i = r; i < (size_t)A.n_seqs * A.table_stride; i += kThreads) A.tables_out[i] = A.tables[i];
 }
-
-__global__ void __launch_bounds__(kThreads)
-pages_extend_small_kernel(int* tables, int* lens, int* refs, const int* add, int* missing, int n_seqs, int table_stride, int n_pages, int page_size) {
-    __shared__ int s_first[kSmallSeqs];   // number of pages wanted by the rows before
-    const int r = threadIdx.x;
-    const int len = r < n_seqs ? max(lens[r], 0) : 0;
-    const long more = r < n_seqs ? max(add[r], 0) : 0;
-    MyPages mine;
-    mine.load(refs, n_pages);
-    const long pages = (len + more + page_size - 1) / page_size;
-    const bool fits = pages <= table_stride && len + more <= 0x7fffffffl;
-    const int held = pages_of(len, page_size, table_stride);
-    int wanted, available;
-    s_first[r] = block_scan(fits ? (int)pages - held : 0, &wanted);
-    const int before = block_scan(mine.free_count(), &available);
-    const bool refused = __syncthreads_or(!fits);
-    if (r == 0) *missing = refused ? -1 : available < wanted ? wanted - available : 0;
-    if (refused || available < wanted) return;
-    mine.take(before, wanted, [&](int k, int page) {
-        int lo = 0, hi = n_seqs - 1;      // the last row whose first page is at most k
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (s_first[mid] <= k) lo = mid;
-            else hi = mid - 1;
-        }
-        refs[page] = 1;
-        tables[(size_t)lo * table_stride + pages_of(lens[lo], page_size, table_stride) + k - s_first[lo]] = page;
-    });
-    __syncthreads();                       // every length has been read
-    if (r < n_seqs) lens[r] = len + (int)more;
-}
-
-// Plan and remap of a small pool.  s_new: a page's new id; the k-th mover and the k-th hole meet in the two lists.
-__global__ void __launch_bounds__(kThreads)
-pages_compact_small_kernel(const int* tables, const int* refs, int* tables_out, int* refs_out, int* remap, int* copy_src, int* copy_dst, int* count,
-                           int n_pages, int n_entries) {
-    __shared__ unsigned short s_mover[kSmallPages / 2], s_hole[kSmallPages / 2];
-    extern __shared__ int s_new[];
-    const int tid = threadIdx.x;
-    MyPages mine;
-    mine.load(refs, n_pages);
-    int live, total, holes;
-    block_scan(mine.count([&](int p, int ref) { return p < n_pages && ref > 0; }), &live);
-    int m = block_scan(mine.count([&](int p, int ref) { return p < n_pages && p >= live && ref > 0; }), &total);
-    int h = block_scan(mine.count([&](int p, int ref) { return p < live && ref <= 0; }), &holes);
-    const int movers = total;              // as many as holes, at most half of the pages
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int p = mine.page(j);
-        if (j < mine.per && p < n_pages) {
-            if (p >= live && mine.ref[j] > 0) s_mover[m++] = (unsigned short)p;
-            if (p < live && mine.ref[j] <= 0) s_hole[h++] = (unsigned short)p;
-            s_new[p] = mine.ref[j] > 0 ? p : -1;
-        }
-    }
-    __syncthreads();
-    for (int k = tid; k < movers; k += kThreads) s_new[s_mover[k]] = s_hole[k];
-    __syncthreads();
-    for (int k = tid; k < n_pages; k += kThreads) {
-        copy_src[k] = k < movers ? s_mover[k] : -1;
-        copy_dst[k] = k < movers ? s_hole[k] : -1;
-        const int to = s_new[k], ref = refs[k];
-        remap[k] = to;
-        if (k >= live) refs_out[k] = 0;
-        if (to >= 0) refs_out[to] = ref;   // below the line: itself, or the hole that it fills
-    }
-    if (tid == 0) *count = movers;
-    for (int i = tid; i < n_entries; i += kThreads) {
-        const int p = tables[i];
-        tables_out[i] = p >= 0 && p < n_pages ? s_new[p] : p;
-    }
-}
-
-// ---- any size ----
 
 __global__ void __launch_bounds__(256) pages_copy_ints_kernel(int* out, const int* in, size_t n) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) out[i] = in[i];
@@ -354,7 +265,9 @@ __global__ void __launch_bounds__(kThreads) pages_fork_take_kernel(ForkArgs A) {
         if (r < A.n_seqs && A.copy_src[r] >= 0) A.copy_dst[k] = r;      // the k-th row that wants a page, for a moment
         wanted += total;
     }
-    const int available = wanted ? count_free(A.refs_out, A.n_pages, wanted) : 0;
+    const PageRange range(A.refs_out, A.n_pages);
+    int before = 0;
+    const int available = wanted ? range.count(is_free, &before) : 0;
     if (threadIdx.x == 0) *A.missing = available < wanted ? wanted - available : 0;
     __syncthreads();
     if (available < wanted) {
@@ -368,7 +281,9 @@ __global__ void __launch_bounds__(kThreads) pages_fork_take_kernel(ForkArgs A) {
     }
     if (wanted == 0) return;
     // The list sits in copy_dst[0, wanted); the pages go to the rows' tables, and copy_dst is filled from there.
-    take_free(A.refs_out, A.n_pages, wanted, [&](int k, int page) {
+    range.visit(before, wanted, is_free, [&](int k, int page, int) {
+        if (k >= wanted) return;
+        A.refs_out[page] = 1;
         const int row = A.copy_dst[k];
         A.tables_out[(size_t)row * A.table_stride + pages_of(A.lens_out[row], A.page_size, A.table_stride) - 1] = page;
     });
@@ -387,9 +302,9 @@ pages_extend_kernel(int* tables, int* lens, int* refs, const int* add, int* miss
         int need = 0;
         if (r < n_seqs) {
             const int len = max(lens[r], 0);
-            const long more = max(add[r], 0);
-            const long pages = (len + more + page_size - 1) / page_size;
-            if (pages > table_stride || len + more > 0x7fffffffl) refused = 1;
+            const unsigned target = (unsigned)len + (unsigned)max(add[r], 0);
+            const unsigned pages = target ? (target - 1) / (unsigned)page_size + 1 : 0;
+            if (target > 0x7fffffffu || pages > (unsigned)table_stride) refused = 1;
             else need = (int)pages - pages_of(len, page_size, table_stride);
         }
         int total;
@@ -398,11 +313,15 @@ pages_extend_kernel(int* tables, int* lens, int* refs, const int* add, int* miss
         wanted += total;
     }
     refused = __syncthreads_or(refused);
-    const int available = count_free(refs, n_pages, wanted);
+    const PageRange range(refs, n_pages);
+    int before = 0;
+    const int available = wanted ? range.count(is_free, &before) : 0;      // often no sequence needs a page
     if (threadIdx.x == 0) *missing = refused ? -1 : available < wanted ? wanted - available : 0;
     if (refused || available < wanted) return;
     __syncthreads();
-    take_free(refs, n_pages, wanted, [&](int k, int page) {
+    range.visit(before, wanted, is_free, [&](int k, int page, int) {
+        if (k >= wanted) return;
+        refs[page] = 1;
         int lo = 0, hi = n_seqs - 1;      // the last row whose first page is at most k
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -431,47 +350,37 @@ pages_free_kernel(int* tables, int* lens, int* refs, const uint8_t* rows, int ta
 }
 
 // One workgroup: the live pages above the number of live pages move into the free ones below it, in page order.
-__global__ void __launch_bounds__(kThreads)
-pages_compact_plan_kernel(const int* refs, int* refs_out, int* remap, int* copy_src, int* copy_dst, int* count, int n_pages) {
-    int live = 0;
-    for (int p0 = 0; p0 < n_pages; p0 += 4 * kThreads) {
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int p = p0 + (int)threadIdx.x * 4 + j;
-            mine += p < n_pages && refs[p] > 0;
-        }
-        int total;
-        block_scan(mine, &total);
-        live += total;
-    }
-    int movers = 0, holes = 0;
-    for (int p0 = 0; p0 < n_pages; p0 += kThreads) {
-        const int p = p0 + (int)threadIdx.x;
-        const int ref = p < n_pages ? refs[p] : 0;
-        const bool mover = ref > 0 && p >= live, hole = p < live && ref <= 0;
-        int total;
-        const int k = movers + block_scan(mover, &total);
-        movers += total;
-        const int h = holes + block_scan(hole, &total);
-        holes += total;
-        if (mover) copy_src[k] = p;
-        if (hole) copy_dst[h] = p;
-        if (p < n_pages) {
-            remap[p] = ref > 0 ? p : -1;
-            refs_out[p] = p < live ? ref : 0;
-        }
-    }
-    __syncthreads();
-    for (int k = threadIdx.x; k < n_pages; k += kThreads) {
-        if (k < movers) {
-            remap[copy_src[k]] = copy_dst[k];
-            refs_out[copy_dst[k]] = refs[copy_src[k]];
-        } else {
-            copy_src[k] = copy_dst[k] = -1;
-        }
-    }
+__global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(const int* refs, int* copy_src, int* copy_dst, int* count, int n_pages) {
+    const PageRange range(refs, n_pages);
+    int before, holes_before;
+    const int live = range.count([](int, int ref) { return ref > 0; }, &before);
+    auto mover = [live](int p, int ref) { return ref > 0 && p >= live; };
+    auto hole = [live](int p, int ref) { return ref <= 0 && p < live; };
+    const int movers = range.count(mover, &before);
+    range.count(hole, &holes_before);
+    range.visit(before, 0x7fffffff, mover, [&](int k, int p, int) { copy_src[k] = p; });
+    range.visit(holes_before, 0x7fffffff, hole, [&](int k, int p, int) { copy_dst[k] = p; });
     if (threadIdx.x == 0) *count = movers;
+}
+// New ids and counts, and the rest of the lists.  The lists are in page order, so the first mover and the last hole tell a
+// page's part: live and not below the first mover, it moves; free and not above the last hole, it is filled.
+__global__ void __launch_bounds__(256)
+pages_compact_apply_kernel(const int* refs, int* refs_out, int* remap, int* copy_src, int* copy_dst, const int* count, int n_pages) {
+    const int movers = *count;
+    const int first = movers ? copy_src[0] : n_pages, last = movers ? copy_dst[movers - 1] : -1;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)n_pages; i += (size_t)gridDim.x * 256) {
+        const int p = (int)i, ref = refs[p];
+        if (ref <= 0) remap[p] = -1;
+        else if (p < first) remap[p] = p;
+        if (p < first && ref > 0) refs_out[p] = ref;
+        else if (p > last || ref > 0) refs_out[p] = 0;
+        if (p < movers) {
+            remap[copy_src[p]] = copy_dst[p];
+            refs_out[copy_dst[p]] = refs[copy_src[p]];
+        } else {
+            copy_src[p] = copy_dst[p] = -1;
+        }
+    }
 }
 
 __global__ void __launch_bounds__(256) pages_remap_kernel(int* out, const int* in, const int* remap, int n_pages, size_t n) {
@@ -520,6 +429,7 @@ pages_copy_kernel(unsigned char* pool, size_t plane_stride, size_t page_stride, 
 static int check_state(const char* what, int n_seqs, int table_stride, int n_pages, int page_size) {
     TL_REQUIRE(n_seqs >= 0 && table_stride >= 1 && n_pages >= 1 && page_size >= 1, "%s: sizes out of range", what);
     if (n_seqs > kMaxSeqs) return set_error(TL_ELIMIT, "%s: %d sequences, at most %d", what, n_seqs, kMaxSeqs);
+    if (n_pages > kMaxPages) return set_error(TL_ELIMIT, "%s: %d pages, at most %d", what, n_pages, kMaxPages);
     if ((size_t)n_seqs * (size_t)table_stride >= (1u << 31)) return set_error(TL_ELIMIT, "%s: tables of %d x %d entries are too large", what, n_seqs, table_stride);
     return TL_OK;
 }
@@ -574,11 +484,6 @@ int tl_pages_extend(int* tables, int* lens, int* refs, const int* add, int* miss
     if (rc != TL_OK) return rc;
     TL_REQUIRE(refs && missing && (n_seqs == 0 || (tables && lens && add)), "%s: null pointer", what);
     TL_ENSURE_INIT();
-    if (small_state(n_seqs, 1, n_pages)) {
-        pages_extend_small_kernel<<<1, kThreads, 0, stream()>>>(tables, lens, refs, add, missing, n_seqs, table_stride, n_pages, page_size);
-        TL_CHECK_LAUNCH("pages_extend_small_kernel");
-        return TL_OK;
-    }
     pages_extend_kernel<<<1, kThreads, (size_t)n_seqs * sizeof(int), stream()>>>(tables, lens, refs, add, missing, n_seqs, table_stride, n_pages, page_size);
     TL_CHECK_LAUNCH("pages_extend_kernel");
     return TL_OK;
@@ -602,17 +507,14 @@ int tl_pages_compact(const int* tables, const int* refs, int* tables_out, int* r
     using namespace tl;
     const char* what = "tl_pages_compact";
     TL_REQUIRE(n_seqs >= 0 && table_stride >= 1 && n_pages >= 1, "%s: sizes out of range", what);
+    if (n_pages > kMaxPages) return set_error(TL_ELIMIT, "%s: %d pages, at most %d", what, n_pages, kMaxPages);
     TL_REQUIRE(refs && refs_out && remap && copy_src && copy_dst && count && (n_seqs == 0 || (tables && tables_out)), "%s: null pointer", what);
     TL_REQUIRE(refs_out != refs, "%s: the new reference counts must not lie over the old ones", what);
     TL_ENSURE_INIT();
-    if (small_state(0, 1, n_pages) && (size_t)n_seqs * (size_t)table_stride <= kSmallEntries) {
-        pages_compact_small_kernel<<<1, kThreads, n_pages * sizeof(int), stream()>>>(tables, refs, tables_out, refs_out, remap, copy_src, copy_dst, count,
-                                                                                    n_pages, n_seqs * table_stride);
-        TL_CHECK_LAUNCH("pages_compact_small_kernel");
-        return TL_OK;
-    }
-    pages_compact_plan_kernel<<<1, kThreads, 0, stream()>>>(refs, refs_out, remap, copy_src, copy_dst, count, n_pages);
+    pages_compact_plan_kernel<<<1, kThreads, 0, stream()>>>(refs, copy_src, copy_dst, count, n_pages);
     TL_CHECK_LAUNCH("pages_compact_plan_kernel");
+    pages_compact_apply_kernel<<<ints_grid(n_pages), 256, 0, stream()>>>(refs, refs_out, remap, copy_src, copy_dst, count, n_pages);
+    TL_CHECK_LAUNCH("pages_compact_apply_kernel");
     const size_t n = (size_t)n_seqs * table_stride;
     if (n > 0) {
         pages_remap_kernel<<<ints_grid(n), 256, 0, stream()>>>(tables_out, tables, remap, n_pages, n);

@@ -356,7 +356,7 @@ def state(rows, page, width, seed, spare, lens=None):
     return tables, lens, refs, rng
 
 
-@pytest.mark.parametrize("rows,page,width,spare", [(1, 16, 4, 2), (4, 16, 8, 8), (7, 5, 3, 20), (64, 16, 40, 70), (300, 8, 9, 400), (1100, 8, 5, 1500), (3, 1, 50, 9), (130, 16, 300, 5000)])
+@pytest.mark.parametrize("rows,page,width,spare", [(1, 16, 4, 2), (4, 16, 8, 8), (7, 5, 3, 20), (64, 16, 40, 70), (300, 8, 9, 400), (1100, 8, 5, 1500), (3, 1, 50, 9), (130, 16, 300, 5000), (40, 1, 2000, 90000)])
 def test_fork_and_extend(dev, rows, page, width, spare):
     tables, lens, refs, rng = state(rows, page, width, rows, spare)
     parents = rng.randint(0, rows, rows)
@@ -436,7 +436,7 @@ def test_free(dev):
     assert np.array_equal(r.cpu().numpy(), np.bincount(tables[tables >= 0], minlength=len(refs)))
 
 
-@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (10, 10), (10, 0), (100, 37), (1024, 512), (5000, 4999), (4097, 1), (20000, 9000)])
+@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (10, 10), (10, 0), (100, 37), (1024, 512), (5000, 4999), (4097, 1), (20000, 9000), (16384, 16383), (16385, 8000), (131072, 70000)])
 def test_compact(dev, n_pages, live):
     rng = np.random.RandomState(n_pages + live)
     refs = np.zeros(n_pages, np.int64)

@@ -15,8 +15,8 @@
 // where every candidate counts those before it: its rank is its place in the answer.  A list that overflows (values in
 // an order that defeats the bound) is given up for n rounds of a maximum over the workgroup.
 //
-// 24 requests of 8 beams over 100003 tokens: 17 + 6 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
-// for 8 us of the first launch, and its workgroups do not all run at a time).  1 request of 4 beams over 32000: 5 + 4 us,
+// 24 requests of 8 beams over 100003 tokens: 16 + 6 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
+// for 8 us of the first launch, and its workgroups do not all run at a time).  1 request of 4 beams over 32000: 4 + 4 us,
 // two launches and their memory latencies.
 #include <cmath>
 
@@ -34,7 +34,7 @@ constexpr int kList = 1024;
 
 struct SliceStats {
     double sum;                                           // of 2^(logit log2 e - top), NaN if the slice holds NaN or +inf
-    float top;                                            // largest logit times log2 e, as rounded; -inf: nothing but -inf
+    float top;                                            // a whole number, kLowest for nothing but -inf
     float pad;
 };
 
@@ -65,30 +65,42 @@ __device__ __forceinline__ float candidate_logit(unsigned c) {
 }
 __device__ __forceinline__ int candidate_index(unsigned c) { return (1 << kIndexBits) - 1 - (int)(c & ((1u << kIndexBits) - 1)); }
 
-// v of the lane with one bit of its number flipped, for values that are equal within groups of 2^BIT adjacent lanes (what the
-// steps of a reduction over lanes leave behind): within 16 lanes by moves in the vector pipe, not through LDS.
-template <int BIT, class T>
-__device__ __forceinline__ T other_half(T v) {
-    if constexpr (BIT >= 4) {
-        return __shfl_xor(v, 1 << BIT, 64);
+// One step of a reduction over lanes whose f does not care for the order of its operands: v joined with the value of the lane
+// whose number differs in one bit, for values that are equal within groups of 2^BIT adjacent lanes (what the steps before
+// leave behind).  All in the vector pipe: quads, mirrored halves of 8 and 16, then swapped rows of 16 and 32.
+template <int BIT, class F>
+__device__ __forceinline__ unsigned join_word(unsigned v, F f) {
+    if constexpr (BIT < 4) {
+        constexpr int ctrl = BIT == 0 ? 0xB1 : BIT == 1 ? 0x4E : BIT == 2 ? 0x141 : 0x140;
+        return f(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true));
     } else {
-        constexpr int ctrl = BIT == 0 ? 0xB1 : BIT == 1 ? 0x4E : BIT == 2 ? 0x141 : 0x140;     // quads, then mirrored halves
-        if constexpr (sizeof(T) == 4) {
-            return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true));
-        } else {
-            const int2 w = __builtin_bit_cast(int2, v);
-            return __builtin_bit_cast(T, int2{__builtin_amdgcn_update_dpp(0, w.x, ctrl, 0xf, 0xf, true), __builtin_amdgcn_update_dpp(0, w.y, ctrl, 0xf, 0xf, true)});
-        }
+        const auto r = BIT == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return f(r[0], r[1]);
+    }
+}
+template <int BIT, class T, class F>
+__device__ __forceinline__ T join(T v, F f) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, join_word<BIT>(__builtin_bit_cast(unsigned, v), [&](unsigned a, unsigned b) {
+            return __builtin_bit_cast(unsigned, f(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b)));
+        }));
+    } else {
+        const uint2 w = __builtin_bit_cast(uint2, v);
+        unsigned other;
+        const unsigned x = join_word<BIT>(w.x, [&](unsigned a, unsigned b) { other = b; return a; });
+        unsigned other_y;
+        const unsigned y = join_word<BIT>(w.y, [&](unsigned a, unsigned b) { other_y = b; return a; });
+        return f(__builtin_bit_cast(T, uint2{x, y}), __builtin_bit_cast(T, uint2{other, other_y}));
     }
 }
 template <class T, class F>
 __device__ __forceinline__ T over_wave(T v, F f) {
-    v = f(v, other_half<0>(v), 0);
-    v = f(v, other_half<1>(v), 1);
-    v = f(v, other_half<2>(v), 2);
-    v = f(v, other_half<3>(v), 3);
-    v = f(v, other_half<4>(v), 4);
-    return f(v, other_half<5>(v), 5);
+    v = join<0>(v, [&](T a, T b) { return f(a, b, 0); });
+    v = join<1>(v, [&](T a, T b) { return f(a, b, 1); });
+    v = join<2>(v, [&](T a, T b) { return f(a, b, 2); });
+    v = join<3>(v, [&](T a, T b) { return f(a, b, 3); });
+    v = join<4>(v, [&](T a, T b) { return f(a, b, 4); });
+    return join<5>(v, [&](T a, T b) { return f(a, b, 5); });
 }
 template <class T>
 __device__ __forceinline__ T wave_max(T v) {
@@ -122,6 +134,8 @@ __device__ __forceinline__ unsigned order_of(float f) {
 __device__ __forceinline__ float from_order(unsigned o) { return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu)); }
 
 constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.925963033500011e-8f;      // the sum is log2 e to 2^-49
+constexpr float kLowest = -131072.f;                      // below every finite half times log2 e
+__device__ __forceinline__ int exponent_of(float c, float reference) { return (int)fmaxf(c - reference, -1024.f); }
 
 // NV: 16-byte pieces of logits per thread; a slice is NV * 2048 of them.
 template <int NV>
@@ -130,7 +144,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
     static_assert(SLICE <= 1 << kIndexBits, "index bits");
     __shared__ __align__(16) unsigned s_list[kList];
     __shared__ unsigned s_bound[kBeamWaves], s_share[kBeamWaves], s_best[kBeamWaves];
-    __shared__ half_t s_top[kBeamWaves];
+    __shared__ float s_c[kBeamWaves];
     __shared__ double s_sum[kBeamWaves];
     __shared__ int s_count;
     const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, wave = tid / 64;
@@ -150,8 +164,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
         }
     }
     if (tid == 0) s_count = 0;
-    // the largest logit of each piece and of the thread; NaN shows in the sum
+    // Piece by piece as they arrive: its largest logit, and the sum of 2^(x log2 e - c) with a whole number c of its own, so that
+    // sums with other c join without rounding.  A piece of -inf has a c below all others and a sum of 0; NaN and +inf show
+    // as NaN.
     half_t most[NV], top = (half_t)-INFINITY;
+    float part[NV], c[NV], c_thread = kLowest;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         half2_t m[4];
@@ -160,7 +177,19 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
         m[0] = __builtin_elementwise_max(__builtin_elementwise_max(m[0], m[1]), __builtin_elementwise_max(m[2], m[3]));
         most[j] = __builtin_elementwise_max(m[0][0], m[0][1]);
         top = __builtin_elementwise_max(top, most[j]);
+        c[j] = fmaxf(ceilf((float)most[j] * kLog2eHi), kLowest);
+        c_thread = fmaxf(c_thread, c[j]);
+        float p[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = (float)v[j][e];
+            p[e % 2] += __builtin_amdgcn_exp2f(__builtin_fmaf(f, kLog2eLo, __builtin_fmaf(f, kLog2eHi, -c[j])));
+        }
+        part[j] = p[0] + p[1];
     }
+    float mine_sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) mine_sum += ldexpf(part[j], exponent_of(c[j], c_thread));
     int first = NV - 1;                                   // the first piece that holds it
 #pragma unroll
     for (int j = NV - 2; j >= 0; --j)
@@ -169,59 +198,51 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
     const unsigned mine_least = candidate(top, (first * kBeamThreads + tid) * 8 + 7);
     const unsigned bound = smallest_group_maximum(mine_least, A.groups_log2);
     const unsigned share = smallest_group_maximum(mine_least, A.groups_log2 > 2 ? A.groups_log2 - 2 : 0);
-    const float wave_top = wave_max((float)top);
+    const float c_wave = wave_max(c_thread);
+    const double sum_wave = wave_sum((double)ldexpf(mine_sum, exponent_of(c_thread, c_wave)));
     if (tid % 64 == 0) {
         s_bound[wave] = bound;
         s_share[wave] = share;
-        s_top[wave] = (half_t)wave_top;
+        s_c[wave] = c_wave;
+        s_sum[wave] = sum_wave;
     }
     __syncthreads();
     unsigned reach = 0, all = ~0u;
-    float slice_top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kBeamWaves; ++w) {
         reach = max(reach, s_bound[w]);
         all = min(all, s_share[w]);
-        slice_top = fmaxf(slice_top, (float)s_top[w]);
     }
     reach = max(reach, all);
-    // sum of 2^(x log2 e - c) with c as it was rounded: the logarithm gets exactly that c back
-    const float c = slice_top == -INFINITY ? 0.f : slice_top * kLog2eHi;
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        float part[2] = {0.f, 0.f};                       // four terms each, then fp64
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float f = (float)v[j][e];
-            part[e % 2] += __builtin_amdgcn_exp2f(__builtin_fmaf(f, kLog2eLo, __builtin_fmaf(f, kLog2eHi, -c)));   // -inf: 0
-        }
-        sum += (double)part[0] + (double)part[1];
+    if (tid == 0) {
+        float c_slice = kLowest;
+        double sum = 0.0;
+        for (int w = 0; w < kBeamWaves; ++w) c_slice = fmaxf(c_slice, s_c[w]);
+        for (int w = 0; w < kBeamWaves; ++w) sum += ldexp(s_sum[w], exponent_of(s_c[w], c_slice));
+        A.stats[(size_t)row * A.n_slices + slice] = {sum, c_slice, 0.f};
     }
     // what reaches the bound
     const half_t reach_value = (half_t)candidate_logit(reach);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         if (!(most[j] >= reach_value)) continue;
+        unsigned hits = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (!(v[j][e] >= reach_value)) continue;
+        for (int e = 0; e < 8; ++e) hits |= v[j][e] >= reach_value ? 1u << e : 0u;
+        const uint4 w = __builtin_bit_cast(uint4, v[j]);
+        while (hits) {                                    // one or two lanes, once, as a rule
+            const int e = __builtin_ctz(hits);
+            hits &= hits - 1;
+            const unsigned pair = e < 4 ? (e < 2 ? w.x : w.y) : (e < 6 ? w.z : w.w);
             const int i = (j * kBeamThreads + tid) * 8 + e;
-            const unsigned cand = candidate(v[j][e], i);
+            const unsigned cand = candidate(__builtin_bit_cast(half_t, (unsigned short)(pair >> (e % 2 * 16))), i);
             if (cand >= reach && i < n) {
                 const int at = atomicAdd(&s_count, 1);
                 if (at < kList) s_list[at] = cand;
             }
         }
     }
-    sum = wave_sum(sum);
-    if (tid % 64 == 0) s_sum[wave] = sum;
     __syncthreads();
-    if (tid == 0) {
-        sum = 0.0;
-        for (int w = 0; w < kBeamWaves; ++w) sum += s_sum[w];
-        A.stats[(size_t)row * A.n_slices + slice] = {slice_top < INFINITY ? sum : (double)NAN, slice_top == -INFINITY ? -INFINITY : c, 0.f};
-    }
     unsigned* best = A.best + ((size_t)row * A.n_slices + slice) * A.n_select;
     const int count = s_count;
     if (count <= kList) {
@@ -382,10 +403,10 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
             int rank = 0;
             for (int k = tid % parts; k < count; k += parts) rank += better(s_list[k], c);
             if (parts >= 4) {
-                rank += other_half<0>(rank);
-                rank += other_half<1>(rank);
+                rank = join<0>(rank, [](int a, int b) { return a + b; });
+                rank = join<1>(rank, [](int a, int b) { return a + b; });
             }
-            if (parts == 8) rank += other_half<2>(rank);
+            if (parts == 8) rank = join<2>(rank, [](int a, int b) { return a + b; });
             if (tid % parts == 0 && rank < A.n_select) put(rank, c);
         }
         return;

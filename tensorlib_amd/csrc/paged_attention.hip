@@ -50,6 +50,19 @@ struct PagedAttnArgs {
     float scale_log2;
 };
 
+// f over the four lanes of a column (16 and 32 apart), by swapping rows of lanes in the vector pipe.  (The elements are copied
+// out of the returned vector first: a bit cast of an element itself reads element 0.)
+template <class F>
+__device__ __forceinline__ float over_column(float v, F f) {
+    const unsigned a = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    const unsigned b = __builtin_bit_cast(unsigned, f(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1)));
+    const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const unsigned q0 = q[0], q1 = q[1];
+    return f(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
+}
+
 // LDS: the offsets of the chunk's positions, then every wavefront's weighted values of every head of the tile.
 template <int DP>
 static size_t attention_lds(int chunk, int group) {
@@ -207,8 +220,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
                 p[u][r] = t + 16 * u + 4 * grp + r < n ? sc[u][r] * A.scale_log2 : -INFINITY;
                 mx = fmaxf(mx, p[u][r]);
             }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        mx = over_column(mx, [](float a, float b) { return fmaxf(a, b); });
         const float m_new = fmaxf(m, mx);
         const float base = m_new == -INFINITY ? 0.f : m_new;   // a column of -inf so far has weights of zero
         const float alpha = __builtin_amdgcn_exp2f(m - base);
@@ -265,8 +277,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
     }
 
     // join the wavefronts: lane (col, grp) holds head col, dims (4 grp + r) * VD + i
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = over_column(l, [](float a, float b) { return a + b; });
     if (grp == 0) {
         s_ml[wave][0][col] = m;
         s_ml[wave][1][col] = bad ? NAN : l;

@@ -11,6 +11,8 @@ ROOT = os.path.dirname(_PKG)
 CSRC = os.path.join(_PKG, "csrc")
 LIB_PATH = os.path.join(_PKG, "lib", "libtensorlib_amd.so")
 HEADER = os.path.join(ROOT, "include", "tensorlib_amd.h")
+FRONT_SRC = os.path.join(_PKG, "torch_front")
+FRONT_PATH = os.path.join(_PKG, "lib", "tensorlib_torch_front.so")
 
 
 class TensorLibError(RuntimeError):
@@ -25,6 +27,16 @@ def build_library(clean: bool = False) -> str:
     if proc.returncode != 0:
         raise RuntimeError("building libtensorlib_amd.so failed:\n" + proc.stdout[-4000:] + proc.stderr[-4000:])
     return LIB_PATH
+
+
+def build_front(clean: bool = False) -> str:
+    """Compile the native Python front end of the serving operators (torch's headers, no GPU needed)."""
+    if clean:
+        subprocess.run(["make", "-C", FRONT_SRC, "clean"], check=True, capture_output=True)
+    proc = subprocess.run(["make", "-C", FRONT_SRC], capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("building tensorlib_torch_front.so failed:\n" + proc.stdout[-3000:] + proc.stderr[-4000:])
+    return FRONT_PATH
 
 
 def declared_symbols() -> list[str]:
@@ -157,6 +169,28 @@ def lib() -> ctypes.CDLL:
         fn.argtypes = args
     _lib = handle
     return _lib
+
+
+_front = None
+
+
+def front():
+    """Load the serving operators' native front end (never builds, never falls back)."""
+    global _front
+    if _front is None:
+        lib()  # the front end binds to the library that is loaded
+        if not os.path.exists(FRONT_PATH):
+            raise TensorLibError(f"{FRONT_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+                                 "or `make -C tensorlib_amd/torch_front`")
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries have to be there first)
+        loader = importlib.machinery.ExtensionFileLoader("tensorlib_torch_front", FRONT_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("tensorlib_torch_front", loader))
+        loader.exec_module(module)
+        _front = module
+    return _front
 
 
 def check(status: int, what: str = "") -> None:

@@ -9,12 +9,13 @@ every computation happens in libtensorlib_amd.so.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import numpy as np
 import torch
 
-from ._lib import KvPages, TensorLibError, check, lib
+from ._lib import TensorLibError, check, front, lib
 
 _OPS = {"add": 0, "sub": 1, "mul": 2, "div": 3}
 # Three attribute look-ups and a Stream object less than torch.cuda.current_stream(), 2.5 us of a 10 us call.
@@ -492,50 +493,7 @@ class HipDevice:
         return out
 
     # -- several sequences over a paged key-value cache --------------------------------
-    # The checks below stand in front of kernels of a few microseconds: one expression each for what is right, and
-    # _refuse() to say what is wrong.
-    def _refuse(self, t, dtype, name, shape, dense=True):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise TensorLibError(f"{name} must be a CUDA(HIP) tensor; there is no CPU path")
-        if t.device.index != self.ordinal:
-            raise ValueError(f"{name} is on {t.device}, this device is cuda:{self.ordinal}")
-        if t.dtype is not dtype:
-            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-        if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-            raise ValueError(f"{name} must have shape {tuple('any' if w is None else w for w in shape)}, got {tuple(t.shape)}")
-        raise ValueError(f"{name} must be contiguous" if dense else f"{name} has unsupported strides {t.stride()}")
-
-    def _arg(self, t, dtype, name, *shape):
-        """Pointer of a contiguous tensor of this device with the given type and shape."""
-        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self.ordinal and t.shape == shape and t.is_contiguous():
-            return t.data_ptr()
-        return self._refuse(t, dtype, name, shape)
-
-    def _any(self, t, dtype, name, dims):
-        """Pointer of a contiguous tensor of this device with the given type and number of dimensions."""
-        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self.ordinal and t.dim() == dims and t.is_contiguous():
-            return t.data_ptr()
-        return self._refuse(t, dtype, name, (None,) * dims)
-
-    def _head_rows(self, t, name, heads=None, dim=None):
-        """Pointer and row stride of [rows, heads, dim] halves whose heads lie next to each other (rows may be apart)."""
-        if isinstance(t, torch.Tensor) and t.dtype is torch.float16 and t.get_device() == self.ordinal and t.dim() == 3:
-            n, h, d = t.shape
-            rs, hs, ds = t.stride()
-            if ((heads is None or h == heads) and (dim is None or d == dim) and (ds == 1 or d <= 1) and (hs == d or h <= 1)
-                    and (rs >= h * d or n <= 1)):
-                return t.data_ptr(), rs
-        return self._refuse(t, torch.float16, name, (None, heads, dim), False)
-
-    def _kv_pages(self, k, v):
-        if isinstance(k, torch.Tensor) and k.dtype is torch.float16 and k.get_device() == self.ordinal and k.dim() == 4:
-            st = k.stride()
-            if (isinstance(v, torch.Tensor) and v.dtype is torch.float16 and v.get_device() == self.ordinal and v.shape == k.shape
-                    and v.stride() == st and (st[3] == 1 or k.shape[3] <= 1)):
-                return KvPages(k.data_ptr(), v.data_ptr(), *st[:3], *k.shape)
-            return self._refuse(v, torch.float16, "v_pages (strides as k_pages, dense heads)", tuple(k.shape), False)
-        return self._refuse(k, torch.float16, "k_pages", (None,) * 4, False)
-
+    # Types, shapes, strides and devices are checked, and results allocated, in torch_front/serving.cpp.
     def _may_allocate(self):
         """Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current
         stream: the library must enqueue on that one, and launch on this device."""
@@ -555,23 +513,21 @@ class HipDevice:
                                              original_context, slow_turns, fast_turns), "tl_rotary_frequencies")
         return self.from_numpy(out)
 
+    @functools.cached_property
+    def _front(self):
+        return front()
+
+    def _layout(self, layout: str) -> int:
+        if layout not in _ROTARY_LAYOUTS:
+            raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
+        return _ROTARY_LAYOUTS[layout]
+
     def rotary(self, x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, layout: str = "half", magnitude: float = 1.0,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """x [tokens, heads, dim] with the first 2 * len(freq) elements of each head rotated to positions[token]; rows may
         be column blocks of a wider matrix. out=x rotates in place."""
-        px, sx = self._head_rows(x, "x")
-        n, h, d = x.shape
-        if layout not in _ROTARY_LAYOUTS:
-            raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
-        pp, pf = self._arg(positions, torch.int32, "positions", n), self._any(freq, torch.float64, "freq", 1)
         self._may_allocate()
-        if out is None:
-            out = torch.empty((n, h, d), dtype=torch.float16, device=x.device)
-        po, so = self._head_rows(out, "out", h, d)
-        if out.shape[0] != n:
-            raise ValueError(f"out must have {n} rows, got {out.shape[0]}")
-        check(self.lib.tl_rotary_f16(po, so, px, sx, pp, pf, 2 * freq.numel(), _ROTARY_LAYOUTS[layout], magnitude, n, h, d), "tl_rotary_f16")
-        return out
+        return self._front.rotary(self.ordinal, x, positions, freq, self._layout(layout), magnitude, out)
 
     def rotary_paged(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor | None,
                      freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, layout: str = "half",
@@ -579,170 +535,56 @@ class HipDevice:
         """Rotated q [tokens, heads, dim]; rotated k and v [tokens, kv heads, dim] go to the pages [pages, positions, kv heads,
         dim] that tables [sequences, ..] names for position positions[t] of sequence seq_ids[t] (None: sequence t; -1: a
         padded token, not stored)."""
-        cache = self._kv_pages(k_pages, v_pages)
-        d = cache.head_dim
-        pq, sq = self._head_rows(q, "q", None, d)
-        n, h, _ = q.shape
-        pk, sk = self._head_rows(k, "k", cache.n_kv_heads, d)
-        pv, sv = self._head_rows(v, "v", cache.n_kv_heads, d)
-        if k.shape[0] != n or v.shape[0] != n:
-            raise ValueError("q, k and v must have the same number of tokens")
-        if layout not in _ROTARY_LAYOUTS:
-            raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
-        pp, pf = self._arg(positions, torch.int32, "positions", n), self._any(freq, torch.float64, "freq", 1)
-        ps = None if seq_ids is None else self._arg(seq_ids, torch.int32, "seq_ids", n)
-        pt = self._any(tables, torch.int32, "tables", 2)
         self._may_allocate()
-        if q_out is None:
-            q_out = q.new_empty((n, h, d))
-            po = q_out.data_ptr()
-        else:
-            po = self._arg(q_out, torch.float16, "q_out", n, h, d)
-        check(self.lib.tl_rotary_kv_pages_f16(po, pq, sq, pk, sk, pv, sv, pp, ps, pf, 2 * freq.numel(), _ROTARY_LAYOUTS[layout], magnitude, n, h,
-                                              cache, pt, tables.shape[1], tables.shape[0]), "tl_rotary_kv_pages_f16")
-        return q_out
+        return self._front.rotary_paged(self.ordinal, q, k, v, positions, seq_ids, freq, k_pages, v_pages, tables, self._layout(layout), magnitude,
+                                        q_out)
 
     def paged_attention(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
                         scale: float | None = None, max_len: int | None = None, out: torch.Tensor | None = None,
                         workspace: torch.Tensor | None = None) -> torch.Tensor:
-        """One token per sequence: q [sequences, heads, dim] attends to the first lens[b] positions of its pages. max_len
-        bounds lens (default: what the tables cover). The workspace is allocated here unless one is passed (uint8, at
-        least paged_attention_workspace(..) bytes, not shared with a call that may overlap)."""
-        cache = self._kv_pages(k_pages, v_pages)
-        d = cache.head_dim
-        pq, sq = self._head_rows(q, "q", None, d)
-        b, h, _ = q.shape
-        pt, pl = self._any(tables, torch.int32, "tables", 2), self._arg(lens, torch.int32, "lens", b)
-        rows, width = tables.shape
-        if rows != b:
-            raise ValueError(f"tables must have {b} rows, got {rows}")
-        if max_len is None:
-            max_len = min(width * cache.page_size, 2 ** 31 - 1)
-        elif not 0 <= max_len < 2 ** 31:
-            raise ValueError(f"max_len {max_len} is out of range")
+        """One token per sequence: q [sequences, heads, dim] attends to the first lens[b] positions of its pages; scale defaults
+        to dim ** -0.5. max_len bounds lens (default: what the tables cover). The workspace is allocated here unless one is
+        passed (uint8, at least paged_attention_workspace(..) bytes, not shared with a call that may overlap)."""
         self._may_allocate()
-        if out is None:
-            out = q.new_empty((b, h, d))
-            po = out.data_ptr()
-        else:
-            po = self._arg(out, torch.float16, "out", b, h, d)
-        pw, size = None, 0
-        if workspace is not None:
-            pw, size = self._any(workspace, torch.uint8, "workspace", 1), workspace.numel()
-        else:
-            size = self.lib.tl_paged_attention_workspace(b, h, cache.n_kv_heads, d, max_len)
-            if size:
-                workspace = lens.new_empty((size + 3) // 4)
-                pw = workspace.data_ptr()
-        check(self.lib.tl_paged_attention_f16(po, pq, sq, cache, pt, width, pl, b, h, max_len, d ** -0.5 if scale is None else scale, pw, size),
-              "tl_paged_attention_f16")
-        return out
+        return self._front.paged_attention(self.ordinal, q, k_pages, v_pages, tables, lens, scale, max_len, out, workspace)
 
     def paged_attention_workspace(self, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int) -> int:
         """Bytes of workspace paged_attention needs for these sizes; 0 where it needs none."""
         return self.lib.tl_paged_attention_workspace(n_seqs, n_heads, n_kv_heads, head_dim, max_len)
 
-    @staticmethod
-    def _int_arrays(like, *sizes):
-        """int32 arrays of these sizes out of one allocation."""
-        return like.new_empty(sum(sizes)).split_with_sizes(sizes)
-
-    def _page_state(self, tables, lens, refs):
-        pt = self._any(tables, torch.int32, "tables", 2)
-        return pt, self._arg(lens, torch.int32, "lens", tables.shape[0]), self._any(refs, torch.int32, "refs", 1)
-
     def pages_fork(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int):
         """Row i of the new state continues sequence parents[i] (-1: empty). Returns (tables, lens, refs, copy_src, copy_dst,
         missing); pages_copy(pool, copy_src, copy_dst) then copies the partly filled pages. missing[0] != 0: not enough
         free pages, the state is unchanged."""
-        pt, pl, pr = self._page_state(tables, lens, refs)
-        n, width = tables.shape
-        pp = self._arg(parents, torch.int32, "parents", n)
         self._may_allocate()
-        t, ln, r, src, dst, missing = self._int_arrays(tables, n * width, n, refs.shape[0], n, n, 1)
-        t = t.view(n, width)
-        check(self.lib.tl_pages_fork(pt, pl, pr, pp, t.data_ptr(), ln.data_ptr(), r.data_ptr(), src.data_ptr(), dst.data_ptr(), missing.data_ptr(),
-                                     n, width, refs.shape[0], page_size), "tl_pages_fork")
-        return t, ln, r, src, dst, missing
+        return self._front.pages_fork(self.ordinal, tables, lens, refs, parents, page_size)
 
     def pages_extend(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, add: torch.Tensor, page_size: int) -> torch.Tensor:
         """Room for add[i] more positions of every sequence, in place. Returns missing ([1]): 0, or why nothing changed."""
-        pt, pl, pr = self._page_state(tables, lens, refs)
-        n, width = tables.shape
-        pa = self._arg(add, torch.int32, "add", n)
         self._may_allocate()
-        missing = tables.new_empty(1)
-        check(self.lib.tl_pages_extend(pt, pl, pr, pa, missing.data_ptr(), n, width, refs.shape[0], page_size), "tl_pages_extend")
-        return missing
+        return self._front.pages_extend(self.ordinal, tables, lens, refs, add, page_size)
 
     def pages_free(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor, page_size: int) -> None:
         """Gives back the pages of the sequences with rows[i] true and empties them, in place."""
-        pt, pl, pr = self._page_state(tables, lens, refs)
-        n, width = tables.shape
-        pw = self._arg(rows, torch.bool, "rows", n)
-        check(self.lib.tl_pages_free(pt, pl, pr, pw, n, width, refs.shape[0], page_size), "tl_pages_free")
+        self._front.pages_free(self.ordinal, tables, lens, refs, rows, page_size)
 
     def pages_compact(self, tables: torch.Tensor, refs: torch.Tensor):
         """Moves the live pages to the low end of the pool. Returns (tables, refs, remap, copy_src, copy_dst, count);
         pages_copy(pool, copy_src, copy_dst, count) then moves the data."""
-        pt, pr = self._any(tables, torch.int32, "tables", 2), self._any(refs, torch.int32, "refs", 1)
         self._may_allocate()
-        n, width = tables.shape
-        pages = refs.shape[0]
-        t, r, remap, src, dst, count = self._int_arrays(tables, n * width, pages, pages, pages, pages, 1)
-        t = t.view(n, width)
-        check(self.lib.tl_pages_compact(pt, pr, t.data_ptr(), r.data_ptr(), remap.data_ptr(), src.data_ptr(), dst.data_ptr(), count.data_ptr(),
-                                        n, width, pages), "tl_pages_compact")
-        return t, r, remap, src, dst, count
+        return self._front.pages_compact(self.ordinal, tables, refs)
 
     def pages_copy(self, pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, count: torch.Tensor | None = None) -> None:
         """pool [planes, pages, ..]: page src[i] of every plane to page dst[i], in place; ids of -1 are skipped, and pairs from
         count[0] on."""
-        if not isinstance(pool, torch.Tensor) or pool.dim() < 3:
-            raise ValueError("pool must be [planes, pages, ...page]")
-        if pool.get_device() != self.ordinal:
-            self._refuse(pool, pool.dtype, "pool", tuple(pool.shape))
-        p = pool.data_ptr()
-        item = pool.element_size()
-        planes, pages, *page = pool.shape
-        plane_stride, page_stride, *inner = pool.stride()
-        page_bytes = item
-        for extent, stride in zip(reversed(page), reversed(inner)):
-            if stride * item != page_bytes and extent > 1:
-                raise ValueError("a page of the pool must be contiguous")
-            page_bytes *= extent
-        ps, pd = self._any(src, torch.int32, "src", 1), self._arg(dst, torch.int32, "dst", src.shape[0])
-        pc = None if count is None else self._arg(count, torch.int32, "count", 1)
-        check(self.lib.tl_pages_copy(p, plane_stride * item, page_stride * item, page_bytes, planes, pages, ps, pd, pc, src.shape[0]),
-              "tl_pages_copy")
+        self._front.pages_copy(self.ordinal, pool, src, dst, count)
 
     def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, n_beams: int, finished: torch.Tensor | None = None, end_token: int = 2,
                     n_select: int | None = None, workspace: torch.Tensor | None = None):
         """logits [requests * n_beams, vocab] (rows may be apart), scores (float32) and finished (bool) per row. Returns the best
         n_select (default n_beams) continuations of every request as flat (scores, tokens, parents), best first."""
-        if not (isinstance(logits, torch.Tensor) and logits.dtype is torch.float16 and logits.get_device() == self.ordinal and logits.dim() == 2):
-            self._refuse(logits, torch.float16, "logits", (None, None), False)
-        pl = logits.data_ptr()
-        rows, vocab = logits.shape
-        row_stride, one = logits.stride()
-        if n_beams < 1 or rows % n_beams or one != 1 and vocab > 1 or row_stride < vocab and rows > 1:
-            raise ValueError(f"logits must be [requests * {n_beams}, vocab] with dense rows, got {tuple(logits.shape)}, strides {logits.stride()}")
-        ps = self._arg(scores, torch.float32, "scores", rows)
-        pf = None if finished is None else self._arg(finished, torch.bool, "finished", rows)
-        batch, n = rows // n_beams, n_beams if n_select is None else n_select
         self._may_allocate()
-        out = scores.new_empty(max(batch * n, 0))
-        ints = torch.empty((2, max(batch * n, 0)), dtype=torch.int32, device=logits.device)
-        tokens, parents = ints.unbind()
-        if workspace is None:
-            size = self.lib.tl_beam_select_workspace(batch, n_beams, vocab, n)
-            workspace = scores.new_empty((size + 3) // 4)
-            pw = workspace.data_ptr()
-        else:
-            pw, size = self._any(workspace, torch.uint8, "workspace", 1), workspace.numel()
-        check(self.lib.tl_beam_select_f16(out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), pl, row_stride, ps, pf, batch, n_beams, vocab, n,
-                                          end_token, pw, size), "tl_beam_select_f16")
-        return out, tokens, parents
+        return self._front.beam_select(self.ordinal, logits, scores, n_beams, finished, end_token, n_select, workspace)
 
     def beam_select_workspace(self, n_batch: int, n_beams: int, vocab: int, n_select: int) -> int:
         """Bytes of workspace beam_select needs for these sizes."""
@@ -752,18 +594,8 @@ class HipDevice:
                      tokens: torch.Tensor, end_token: int = 2):
         """The histories [rows, width] after a selection: row i is parents[i]'s with tokens[i] behind it. Returns (history, lens,
         finished)."""
-        ph = self._any(history, torch.int32, "history", 2)
-        rows, width = history.shape
-        pl = self._arg(lens, torch.int32, "lens", rows)
-        pf = None if finished is None else self._arg(finished, torch.bool, "finished", rows)
-        pp = self._any(parents, torch.int32, "parents", 1)
-        n = parents.shape[0]
-        pt = self._arg(tokens, torch.int32, "tokens", n)
         self._may_allocate()
-        h, ln = history.new_empty((n, width)), lens.new_empty(n)
-        f = torch.empty(n, dtype=torch.bool, device=history.device) if finished is None else finished.new_empty(n)
-        check(self.lib.tl_beam_advance(h.data_ptr(), ln.data_ptr(), f.data_ptr(), ph, pl, pf, pp, pt, rows, n, width, end_token), "tl_beam_advance")
-        return h, ln, f
+        return self._front.beam_advance(self.ordinal, history, lens, finished, parents, tokens, end_token)
 
     # -- tuning hooks -------------------------------------------------------------------
     def set_gemv_variant(self, v: int) -> None:

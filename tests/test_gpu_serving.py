@@ -801,3 +801,66 @@ def test_front_end_refusals(dev):
     with torch.cuda.stream(torch.cuda.Stream()):                   # not the stream the library enqueues on
         with pytest.raises(TensorLibError, match="stream"):
             dev.paged_attention(q, kp, vp, t, ln)
+
+
+def test_results_are_the_callers_own(dev):
+    """Results that share an allocation: apart from each other, usable on their own, alive when the others are gone, and
+    not written by later calls."""
+    for rows, width, pages in ((3, 5, 70), (1, 1, 1), (65, 63, 4096)):
+        tables = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
+        lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+        parents = torch.arange(rows, dtype=torch.int32, device="cuda")
+        first = dev.pages_fork(tables, lens, refs, parents, 4)
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in first)
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+        assert all(t.is_contiguous() and not t.requires_grad and t.is_leaf and t._version == 0 for t in first)
+        for i, t in enumerate(first):
+            t.fill_(100 + i)
+        second = dev.pages_fork(tables, lens, refs, parents, 4)
+        assert all(bool((t == 100 + i).all()) for i, t in enumerate(first))
+        kept = second[2]
+        del second
+        other = [torch.full((pages,), 7, dtype=torch.int32, device="cuda") for _ in range(8)]
+        assert not kept.any() and all(bool((t == 7).all()) for t in other)
+    with torch.inference_mode():
+        history = torch.zeros((4, 8), dtype=torch.int32, device="cuda")
+        lens = torch.zeros(4, dtype=torch.int32, device="cuda")
+        ids = torch.arange(4, dtype=torch.int32, device="cuda")
+        h2, l2, f2 = dev.beam_advance(history, lens, None, ids, ids + 5, end_token=6)
+        assert h2.is_inference() and h2[:, 0].tolist() == [5, 6, 7, 8] and l2.tolist() == [1] * 4
+        assert f2.dtype == torch.bool and f2.tolist() == [False, True, False, False]
+    h2, l2, f2 = dev.beam_advance(history, lens, f2, ids, ids, end_token=6)
+    assert f2.logical_not().tolist() == [True, False, True, True]
+
+
+def test_calls_from_several_threads(dev):
+    """The library's errors are per thread and a launch runs without the interpreter's lock."""
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((40, 4, 64), generator=g, device="cuda", dtype=torch.float16)
+    positions = torch.arange(40, dtype=torch.int32, device="cuda")
+    freq = dev.rotary_frequencies(64)
+    want = dev.rotary(x, positions, freq)
+    wrong = []
+
+    def right():
+        for _ in range(50):
+            if not torch.equal(dev.rotary(x, positions, freq), want):
+                wrong.append("result")
+
+    def refused():
+        for _ in range(50):
+            try:
+                dev.rotary(x[..., :63].contiguous(), positions, freq)
+                wrong.append("no refusal")
+            except TensorLibError as e:
+                if "tl_rotary_f16" not in str(e):
+                    wrong.append(str(e))
+
+    threads = [threading.Thread(target=t) for t in (right, refused, right)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]

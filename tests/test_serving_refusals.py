@@ -171,3 +171,22 @@ def test_frequencies_follow_the_formulas(rd, base):
 def test_frequencies_refuse(args, match):
     rc, msg, _ = frequencies(**args)
     assert rc == TL_EINVAL and match in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("name,arguments", [
+    ("rotary", 7), ("rotary_paged", 13), ("paged_attention", 10), ("pages_fork", 6), ("pages_extend", 6), ("pages_free", 6),
+    ("pages_compact", 3), ("pages_copy", 5), ("beam_select", 8), ("beam_advance", 7)])
+def test_native_front_end_takes_device_tensors_only(name, arguments):
+    """The checks in front of the library, as far as they need no GPU: nothing but device tensors, all arguments there."""
+    import torch
+    from tensorlib_amd._lib import TensorLibError, front
+    entry = getattr(front(), name)
+    for wrong in (torch.zeros(2, 2), 1.5, None, "x"):
+        with pytest.raises(TensorLibError, match="no CPU path"):
+            entry(0, *[wrong] * (arguments - 1))
+    with pytest.raises(TypeError, match=f"{arguments} arguments"):
+        entry(0)
+    with pytest.raises(TypeError, match=f"{arguments} arguments"):
+        entry()
+    with pytest.raises(TypeError, match="ordinal"):
+        entry("0", *[None] * (arguments - 1))

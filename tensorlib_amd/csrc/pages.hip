@@ -46,16 +46,19 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
 }
 
 // A workgroup of 1024 over the reference counts of any number of pages: each wavefront has a sixteenth of them to itself and
-// goes through it in page order, 256 at a time, so that ranks come from ballots and the wavefronts meet only once.
+// goes through it in page order, 256 at a time, so that ranks come from ballots and the wavefronts meet only once.  The first
+// 256 are read when the range is made, early where that hides the wait, and kept: up to 4096 pages there are no others.
 constexpr int kWaves = kThreads / 64;
 struct PageRange {
     const int* refs;
     int n_pages, begin, end;
+    int4 first;
     __device__ PageRange(const int* refs_, int n_pages_) : refs(refs_), n_pages(n_pages_) {
         const long steps = ((long)n_pages + kWaves * 256 - 1) / (kWaves * 256), wave = threadIdx.x / 64;
         const long b = wave * steps * 256, e = b + steps * 256;
         begin = b < n_pages ? (int)b : n_pages;
         end = e < n_pages ? (int)e : n_pages;
+        first = load(begin + (int)(threadIdx.x % 64) * 4);
     }
     // Four counts of the lane; what lies behind the last page counts as 1, taken and not live: f() never sees it.
     __device__ __forceinline__ int4 load(int p) const {
@@ -69,12 +72,12 @@ struct PageRange {
         return r;
     }
     // take(rank, page, count) for the pages of the wavefront's range that f(page, count) picks, ranks from `rank` on; returns
-    // the rank behind the last one.  Stops at a rank of `most`.
+    // the rank behind the last one.  Stops at a rank of `most`.  Of the counts, take() may change the one it is given.
     template <class F, class T>
     __device__ __forceinline__ int visit(int rank, int most, F f, T take) const {
         const int lane = threadIdx.x % 64;
         const unsigned long long below = (1ull << lane) - 1;
-        int4 next = load(begin + lane * 4);
+        int4 next = first;
         for (int p0 = begin; p0 < end && rank < most; p0 += 256) {
             const int p = p0 + lane * 4;
             const int4 r = next;
@@ -93,107 +96,103 @@ struct PageRange {
         }
         return rank;
     }
-    // How many pages f picks in the whole pool; *before: in the ranges of the wavefronts before this one.
+    // How many pages f picks in the whole pool; *before: in the ranges of the wavefronts before this one.  In the same meeting
+    // the sum of a number `own` of each wavefront, *all_own, and its part before this one, *own_before.
     template <class F>
-    __device__ int count(F f, int* before) const {
-        __shared__ int s_count[kWaves];
+    __device__ int count(F f, int* before, int own, int* own_before, int* all_own) const {
+        __shared__ int2 s_count[kWaves];
         const int n = visit(0, 0x7fffffff, f, [](int, int, int) {});
         __syncthreads();
-        if (threadIdx.x % 64 == 0) s_count[threadIdx.x / 64] = n;
+        if (threadIdx.x % 64 == 0) s_count[threadIdx.x / 64] = {n, own};
         __syncthreads();
         int all = 0;
-        *before = 0;
+        *before = *own_before = *all_own = 0;
+#pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            if (w < (int)threadIdx.x / 64) *before += s_count[w];
-            all += s_count[w];
+            const int2 c = s_count[w];
+            if (w < (int)threadIdx.x / 64) {
+                *before += c.x;
+                *own_before += c.y;
+            }
+            all += c.x;
+            *all_own += c.y;
         }
         return all;
+    }
+    template <class F>
+    __device__ int count(F f, int* before) const {
+        int own_before, all_own;
+        return count(f, before, 0, &own_before, &all_own);
     }
 };
 __device__ __forceinline__ bool is_free(int, int count) { return count == 0; }
 
 constexpr int kSmallPages = 16384;         // a fork of at most this in one launch: the counts fit LDS,
 constexpr int kSmallSeqs = kThreads;       // the rows a thread each,
-constexpr size_t kSmallEntries = 32768;    // and the tables' entries are soon gone through
+constexpr size_t kSmallEntries = 65536;    // and the tables' entries are soon gone through
 
 struct ForkArgs {
     const int *tables, *lens, *refs, *parents;
     int *tables_out, *lens_out, *refs_out, *copy_src, *copy_dst, *missing;
     int n_seqs, table_stride, n_pages, page_size;
-    FastDiv by_vectors;                    // table entries of a row, in steps of VEC
+    int row_shift;                         // log2 of the threads a row has
 };
 
-// A fork in one launch, one workgroup (48 x 4 rows of 128 entries 10 us, against 13 for the three launches below and two more
-// from the host; at 65536 entries 23 against 18).  VEC: table entries a thread moves at a time, 4 where rows are 16-byte
-// aligned.
+// A fork in one launch, one workgroup (192 x 128 entries of which 19 are pages 7.2 us, against 11 for the three launches
+// below; 256 x 128 with 120 pages 15 against 23; 512 x 128 13 against 14.5 and 31 against 33; 1000 x 128 with 60 pages 63
+// against 45).  A row has 1024 / n_seqs threads, rounded down to a power of two.  First the counts: an entry of an old row is
+// named by the row's children instead of by the row, a partly filled last page by the first of them, so nothing changes for
+// a row with one child and its table need not be read.  The new tables are written last, when all pages are known, since a
+// barrier behind a store waits for it (1.4 us).  VEC: table entries a thread moves at a time, 4 where rows are 16-byte aligned.
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) {
-    __shared__ int s_len[kSmallSeqs], s_pages[kSmallSeqs], s_parent[kSmallSeqs], s_first[kSmallSeqs], s_page[kSmallSeqs];
+    __shared__ int s_len[kSmallSeqs], s_pages[kSmallSeqs], s_full[kSmallSeqs], s_parent[kSmallSeqs], s_first[kSmallSeqs], s_children[kSmallSeqs],
+        s_page[kSmallSeqs], s_copy[kSmallSeqs];
     extern __shared__ int s_refs[];
+    struct alignas(4 * VEC) Entries { int v[VEC]; };
     const int r = threadIdx.x;
     const bool row = r < A.n_seqs;
     const int parent = row ? A.parents[r] : -1;
     const int old_len = row ? A.lens[r] : 0;
     for (int p = r; p < A.n_pages; p += kThreads) s_refs[p] = A.refs[p];
+    const int held = pages_of(old_len, A.page_size, A.table_stride);
     s_first[r] = kSmallSeqs;
+    s_children[r] = 0;
     s_len[r] = old_len > 0 ? old_len : 0;
-    s_pages[r] = pages_of(old_len, A.page_size, A.table_stride);     // once: the divisions would be half of the loop below
+    s_pages[r] = held;
+    s_full[r] = old_len > 0 && old_len % A.page_size != 0 ? held - 1 : held;
     s_parent[r] = parent >= 0 && parent < A.n_seqs ? parent : -1;
     __syncthreads();
     const bool has = s_parent[r] >= 0;
     const int len = has ? s_len[parent] : 0;
     const int new_pages = has ? s_pages[parent] : 0;
-    const bool partial = len % A.page_size != 0;
+    const bool partial = has && s_full[parent] < new_pages;
     int last = -1;                         // the page to be copied, if the row is not its parent's first
+    if (has) atomicAdd(s_children + parent, 1);
     if (partial) {
         last = A.tables[(size_t)parent * A.table_stride + new_pages - 1];
         atomicMin(s_first + parent, r);
     }
     __syncthreads();
-    const bool copied = partial && s_first[parent] != r;
-    if (copied) s_page[r] = -2;            // not counted and not written below
-    else s_page[r] = -1;
-    __syncthreads();
-    const unsigned total = (unsigned)A.n_seqs * A.by_vectors.d;
-    for (unsigned i = r; i < total; i += kThreads) {
-        unsigned c;
-        const unsigned to = A.by_vectors.divmod(i, c);
-        c *= VEC;
-        const int from = s_parent[to];
-        const int old_pages = s_pages[to];
-        const int pages = from >= 0 ? s_pages[from] : 0;
-        const int kept = s_page[to] == -2 ? pages - 1 : pages;
-        int o[VEC], x[VEC];
+    const bool wants = partial && s_first[parent] != r && last >= 0 && last < A.n_pages;
+    const int to = r >> A.row_shift, step = VEC << A.row_shift, c0 = (r & ((1 << A.row_shift) - 1)) * VEC;
+    if (to < A.n_seqs && s_children[to] != 1) {
+        const int children = s_children[to], full = s_full[to], pages = s_pages[to];
+        for (int c = c0; c < pages; c += step) {
+            const Entries o = *reinterpret_cast<const Entries*>(A.tables + (size_t)to * A.table_stride + c);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            o[j] = -1;
-            x[j] = -1;
+            for (int j = 0; j < VEC; ++j) {
+                const int gained = (c + j < full ? children : children ? 1 : 0) - 1;
+                if (c + j < pages && gained != 0 && o.v[j] >= 0 && o.v[j] < A.n_pages) atomicAdd(s_refs + o.v[j], gained);
+            }
         }
-        const int* old_row = A.tables + (size_t)to * A.table_stride + c;
-        const int* new_row = A.tables + (size_t)(from >= 0 ? from : 0) * A.table_stride + c;
-        if constexpr (VEC == 4) {
-            if ((int)c < old_pages) *reinterpret_cast<int4*>(o) = *reinterpret_cast<const int4*>(old_row);
-            if ((int)c < pages) *reinterpret_cast<int4*>(x) = *reinterpret_cast<const int4*>(new_row);
-        } else {
-            if ((int)c < old_pages) o[0] = *old_row;
-            if ((int)c < pages) x[0] = *new_row;
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if ((int)c + j < old_pages && o[j] >= 0 && o[j] < A.n_pages) atomicSub(s_refs + o[j], 1);
-            if ((int)c + j >= pages) x[j] = -1;
-            if ((int)c + j < kept && x[j] >= 0 && x[j] < A.n_pages) atomicAdd(s_refs + x[j], 1);
-        }
-        int* out = A.tables_out + (size_t)to * A.table_stride + c;
-        if constexpr (VEC == 4) *reinterpret_cast<int4*>(out) = *reinterpret_cast<int4*>(x);
-        else *out = x[0];
     }
     __syncthreads();
-    const bool wants = copied && last >= 0 && last < A.n_pages;
-    int wanted, before = 0;
-    const int rank = block_scan(wants, &wanted);
+    const unsigned long long wanting = __ballot(wants);
+    int wanted, before, rank;
     const PageRange range(s_refs, A.n_pages);
-    const int available = wanted ? range.count(is_free, &before) : 0;
+    const int available = range.count(is_free, &before, __popcll(wanting), &rank, &wanted);
+    rank += __popcll(wanting & ((1ull << (r % 64)) - 1));
     const bool enough = available >= wanted;
     if (enough) range.visit(before, wanted, is_free, [&](int k, int page, int) {
         if (k >= wanted) return;
@@ -204,14 +203,26 @@ __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) 
     if (r == 0) *A.missing = enough ? 0 : wanted - available;
     if (row) {
         const int page = wants && enough ? s_page[rank] : -1;
-        if (page >= 0) A.tables_out[(size_t)r * A.table_stride + new_pages - 1] = page;
+        s_copy[r] = page;
         A.copy_src[r] = page >= 0 ? last : -1;
         A.copy_dst[r] = page;
         A.lens_out[r] = enough ? len : old_len;
     }
     for (int p = r; p < A.n_pages; p += kThreads) A.refs_out[p] = enough ? s_refs[p] : A.refs[p];
-    if (!enough)
-        for (size_t i = r; i < (size_t)A.n_seqs * A.table_stride; i += kThreads) A.tables_out[i] = A.tables[i];
+    __syncthreads();
+    if (to >= A.n_seqs) return;
+    const int from = enough ? s_parent[to] : to, page = s_copy[to];
+    const int pages = !enough ? A.table_stride : from >= 0 ? s_pages[from] : 0;
+    for (int c = c0; c < A.table_stride; c += step) {
+        Entries x;
+        if (c < pages) x = *reinterpret_cast<const Entries*>(A.tables + (size_t)from * A.table_stride + c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if (c + j >= pages) x.v[j] = -1;
+            if (page >= 0 && c + j == pages - 1) x.v[j] = page;
+        }
+        *reinterpret_cast<Entries*>(A.tables_out + (size_t)to * A.table_stride + c) = x;
+    }
 }
 
 __global__ void __launch_bounds__(256) pages_copy_ints_kernel(int* out, const int* in, size_t n) {
@@ -292,35 +303,49 @@ __global__ void __launch_bounds__(kThreads) pages_fork_take_kernel(ForkArgs A) {
         A.copy_dst[r] = A.copy_src[r] >= 0 ? A.tables_out[(size_t)r * A.table_stride + pages_of(A.lens_out[r], A.page_size, A.table_stride) - 1] : -1;
 }
 
-// Room for add[r] more positions of every sequence, all or nothing (one workgroup).
+// Room for add[r] more positions of every sequence, all or nothing (one workgroup).  Each wavefront has a sixteenth of the
+// sequences and of the pages, and they meet once.  The pages go into a list first and from there to the rows, a thread each with the
+// search for its row: 1.5 us for 192 rows that want a page each, against 3.6 where a lane's four neighbours were searched for in turn.
+constexpr int kListPages = 8192;           // more are stored where they are found
 __global__ void __launch_bounds__(kThreads)
 pages_extend_kernel(int* tables, int* lens, int* refs, const int* add, int* missing, int n_seqs, int table_stride, int n_pages, int page_size) {
+    __shared__ int s_page[kListPages];
+    __shared__ int s_refused;
     extern __shared__ int s_first[];      // number of pages wanted by the rows before
-    int wanted = 0, refused = 0;
-    for (int r0 = 0; r0 < n_seqs; r0 += kThreads) {
-        const int r = r0 + (int)threadIdx.x;
+    const PageRange range(refs, n_pages);
+    const int lane = threadIdx.x % 64, steps = (n_seqs + kThreads - 1) / kThreads, r0 = (int)threadIdx.x / 64 * steps * 64 + lane;
+    if (threadIdx.x == 0) s_refused = 0;
+    int own = 0;
+    bool refused = false;
+    for (int i = 0; i < steps; ++i) {
+        const int r = r0 + i * 64;
         int need = 0;
         if (r < n_seqs) {
             const int len = max(lens[r], 0);
             const unsigned target = (unsigned)len + (unsigned)max(add[r], 0);
             const unsigned pages = target ? (target - 1) / (unsigned)page_size + 1 : 0;
-            if (target > 0x7fffffffu || pages > (unsigned)table_stride) refused = 1;
+            if (target > 0x7fffffffu || pages > (unsigned)table_stride) refused = true;
             else need = (int)pages - pages_of(len, page_size, table_stride);
         }
-        int total;
-        const int k = wanted + block_scan(need, &total);
-        if (r < n_seqs) s_first[r] = k;
-        wanted += total;
+        int x = need;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int y = __shfl_up(x, d, 64);
+            if (lane >= d) x += y;
+        }
+        if (r < n_seqs) s_first[r] = own + x - need;
+        own += __shfl(x, 63, 64);
     }
-    refused = __syncthreads_or(refused);
-    const PageRange range(refs, n_pages);
-    int before = 0;
-    const int available = wanted ? range.count(is_free, &before) : 0;      // often no sequence needs a page
+    int before, own_before, wanted;
+    const int available = range.count(is_free, &before, own, &own_before, &wanted);
+    if (refused) s_refused = 1;
+    for (int i = 0; i < steps; ++i)
+        if (r0 + i * 64 < n_seqs) s_first[r0 + i * 64] += own_before;
+    __syncthreads();
+    refused = s_refused != 0;
     if (threadIdx.x == 0) *missing = refused ? -1 : available < wanted ? wanted - available : 0;
     if (refused || available < wanted) return;
-    __syncthreads();
-    range.visit(before, wanted, is_free, [&](int k, int page, int) {
-        if (k >= wanted) return;
+    auto place = [&](int k, int page) {
         refs[page] = 1;
         int lo = 0, hi = n_seqs - 1;      // the last row whose first page is at most k
         while (lo < hi) {
@@ -329,8 +354,18 @@ pages_extend_kernel(int* tables, int* lens, int* refs, const int* add, int* miss
             else hi = mid - 1;
         }
         tables[(size_t)lo * table_stride + pages_of(lens[lo], page_size, table_stride) + k - s_first[lo]] = page;
+    };
+    const bool listed = wanted <= kListPages;
+    range.visit(before, wanted, is_free, [&](int k, int page, int) {
+        if (k >= wanted) return;
+        if (listed) s_page[k] = page;
+        else place(k, page);
     });
     __syncthreads();
+    if (listed) {
+        for (int k = threadIdx.x; k < wanted; k += kThreads) place(k, s_page[k]);
+        __syncthreads();                   // lens have been read
+    }
     for (int r = threadIdx.x; r < n_seqs; r += kThreads) lens[r] = max(lens[r], 0) + max(add[r], 0);
 }
 
@@ -457,10 +492,10 @@ int tl_pages_fork(const int* tables, const int* lens, const int* refs, const int
     TL_REQUIRE(n_seqs == 0 || (tables && lens && parents && tables_out && lens_out && copy_src && copy_dst), "%s: null pointer", what);
     TL_REQUIRE((n_seqs == 0 || (tables_out != tables && lens_out != lens)) && refs_out != refs, "%s: the new state must not lie over the old one", what);
     TL_ENSURE_INIT();
-    ForkArgs A{tables, lens, refs, parents, tables_out, lens_out, refs_out, copy_src, copy_dst, missing, n_seqs, table_stride, n_pages, page_size, {}};
+    ForkArgs A{tables, lens, refs, parents, tables_out, lens_out, refs_out, copy_src, copy_dst, missing, n_seqs, table_stride, n_pages, page_size, 0};
     if (small_state(n_seqs, table_stride, n_pages)) {
         const bool vec = table_stride % 4 == 0 && aligned16(tables) && aligned16(tables_out);
-        A.by_vectors = FastDiv((unsigned)(vec ? table_stride / 4 : table_stride));
+        while ((n_seqs << (A.row_shift + 1)) <= kThreads && A.row_shift < 10) ++A.row_shift;
         if (vec) pages_fork_small_kernel<4><<<1, kThreads, n_pages * sizeof(int), stream()>>>(A);
         else pages_fork_small_kernel<1><<<1, kThreads, n_pages * sizeof(int), stream()>>>(A);
         TL_CHECK_LAUNCH("pages_fork_small_kernel");

@@ -393,6 +393,44 @@ def test_fork_and_extend(dev, rows, page, width, spare):
         parents = rng.randint(-1, rows, rows)
 
 
+@pytest.mark.parametrize("rows,width,n_pages", [(1, 9000, 9001), (3, 3000, 16384), (1024, 32, 16384), (1024, 31, 16385), (8192, 3, 30000), (8192, 2, 16383), (2, 8192, 16385),
+                                                (65, 127, 8200)])
+def test_extend_by_prompts_and_fork(dev, rows, width, n_pages):
+    """Room for whole prompts at once, up to more pages than are listed on the way, and forks of what came of it, at the limits of
+    a workgroup's shared memory."""
+    page = 2
+    rng = np.random.RandomState(rows + width)
+    refs = (rng.rand(n_pages) < 0.05).astype(int)                  # pages that somebody else holds
+    tables, lens = np.full((rows, width), -1), np.zeros(rows, int)
+    for most in (1, width, width):
+        free = np.flatnonzero(refs == 0)
+        room = width - -(-lens // page)
+        need = np.minimum(rng.randint(0, most + 1, rows), room)
+        if rows == 1:
+            need[:] = np.minimum(room, most)
+        while need.sum() > len(free):
+            need = need // 2
+        add = np.where(need > 0, need * page - (-lens % page > 0) - rng.randint(0, 2, rows), 0)
+        add = np.where(-(-(lens + add) // page) - -(-lens // page) == need, add, need * page)
+        need = -(-(lens + add) // page) - -(-lens // page)
+        t, ln, r = ints(tables), ints(lens), ints(refs)
+        assert int(dev.pages_extend(t, ln, r, ints(add), page)) == 0
+        ranks = np.cumsum(need) - need
+        for i in range(rows):
+            held = -(-int(lens[i]) // page)
+            tables[i, held:held + need[i]] = free[ranks[i]:ranks[i] + need[i]]
+        refs[free[:need.sum()]] = 1
+        lens = lens + add
+        assert np.array_equal(t.cpu().numpy(), tables) and np.array_equal(r.cpu().numpy(), refs) and np.array_equal(ln.cpu().numpy(), lens)
+    parents = np.where(rng.rand(rows) < 0.3, np.arange(rows), rng.randint(-1, rows, rows))
+    want = fork_by_hand(tables, lens, refs, parents, page)
+    *got, missing = dev.pages_fork(t, ln, r, ints(parents), page)
+    assert (want is None) == (int(missing) > 0)
+    if want is not None:
+        assert np.array_equal(got[0].cpu().numpy(), np.array(want[0]))
+        assert all(np.array_equal(g.cpu().numpy(), np.array(w)) for g, w in zip(got[1:], want[1:]))
+
+
 def test_fork_edges(dev):
     # parents out of range leave empty rows; a page counted by nobody's table stays; entries out of range are passed through
     page = 4

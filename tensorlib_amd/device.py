@@ -18,9 +18,6 @@ import torch
 from ._lib import TensorLibError, check, front, lib
 
 _OPS = {"add": 0, "sub": 1, "mul": 2, "div": 3}
-# Three attribute look-ups and a Stream object less than torch.cuda.current_stream(), 2.5 us of a 10 us call.
-_current_device, _current_raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-_ROTARY_LAYOUTS = {"interleaved": 0, "half": 1}
 _ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
 
 
@@ -493,15 +490,7 @@ class HipDevice:
         return out
 
     # -- several sequences over a paged key-value cache --------------------------------
-    # Types, shapes, strides and devices are checked, and results allocated, in torch_front/serving.cpp.
-    def _may_allocate(self):
-        """Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current
-        stream: the library must enqueue on that one, and launch on this device."""
-        if _current_device() != self.ordinal:
-            raise TensorLibError(f"the current device is cuda:{_current_device()}, this device is cuda:{self.ordinal}")
-        if (self.lib.tl_get_stream() or 0) != _current_raw_stream(self.ordinal):
-            raise TensorLibError("the library stream is not torch's current stream; call bind_stream(torch.cuda.current_stream()) first")
-
+    # Types, shapes, strides, device and stream are checked, and results allocated, in torch_front/serving.cpp.
     def rotary_frequencies(self, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
                            original_context: float = 0.0, slow_turns: float = 1.0, fast_turns: float = 32.0) -> torch.Tensor:
         """Radians per position of each pair, float64 on the device; `scaling` is none, linear, base or parts
@@ -517,17 +506,11 @@ class HipDevice:
     def _front(self):
         return front()
 
-    def _layout(self, layout: str) -> int:
-        if layout not in _ROTARY_LAYOUTS:
-            raise ValueError(f"unknown layout {layout!r}, one of {sorted(_ROTARY_LAYOUTS)}")
-        return _ROTARY_LAYOUTS[layout]
-
     def rotary(self, x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, layout: str = "half", magnitude: float = 1.0,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """x [tokens, heads, dim] with the first 2 * len(freq) elements of each head rotated to positions[token]; rows may
         be column blocks of a wider matrix. out=x rotates in place."""
-        self._may_allocate()
-        return self._front.rotary(self.ordinal, x, positions, freq, self._layout(layout), magnitude, out)
+        return self._front.rotary(self.ordinal, x, positions, freq, layout, magnitude, out)
 
     def rotary_paged(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor | None,
                      freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, layout: str = "half",
@@ -535,8 +518,7 @@ class HipDevice:
         """Rotated q [tokens, heads, dim]; rotated k and v [tokens, kv heads, dim] go to the pages [pages, positions, kv heads,
         dim] that tables [sequences, ..] names for position positions[t] of sequence seq_ids[t] (None: sequence t; -1: a
         padded token, not stored)."""
-        self._may_allocate()
-        return self._front.rotary_paged(self.ordinal, q, k, v, positions, seq_ids, freq, k_pages, v_pages, tables, self._layout(layout), magnitude,
+        return self._front.rotary_paged(self.ordinal, q, k, v, positions, seq_ids, freq, k_pages, v_pages, tables, layout, magnitude,
                                         q_out)
 
     def paged_attention(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
@@ -545,7 +527,6 @@ class HipDevice:
         """One token per sequence: q [sequences, heads, dim] attends to the first lens[b] positions of its pages; scale defaults
         to dim ** -0.5. max_len bounds lens (default: what the tables cover). The workspace is allocated here unless one is
         passed (uint8, at least paged_attention_workspace(..) bytes, not shared with a call that may overlap)."""
-        self._may_allocate()
         return self._front.paged_attention(self.ordinal, q, k_pages, v_pages, tables, lens, scale, max_len, out, workspace)
 
     def paged_attention_workspace(self, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int) -> int:
@@ -556,12 +537,10 @@ class HipDevice:
         """Row i of the new state continues sequence parents[i] (-1: empty). Returns (tables, lens, refs, copy_src, copy_dst,
         missing); pages_copy(pool, copy_src, copy_dst) then copies the partly filled pages. missing[0] != 0: not enough
         free pages, the state is unchanged."""
-        self._may_allocate()
         return self._front.pages_fork(self.ordinal, tables, lens, refs, parents, page_size)
 
     def pages_extend(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, add: torch.Tensor, page_size: int) -> torch.Tensor:
         """Room for add[i] more positions of every sequence, in place. Returns missing ([1]): 0, or why nothing changed."""
-        self._may_allocate()
         return self._front.pages_extend(self.ordinal, tables, lens, refs, add, page_size)
 
     def pages_free(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor, page_size: int) -> None:
@@ -571,7 +550,6 @@ class HipDevice:
     def pages_compact(self, tables: torch.Tensor, refs: torch.Tensor):
         """Moves the live pages to the low end of the pool. Returns (tables, refs, remap, copy_src, copy_dst, count);
         pages_copy(pool, copy_src, copy_dst, count) then moves the data."""
-        self._may_allocate()
         return self._front.pages_compact(self.ordinal, tables, refs)
 
     def pages_copy(self, pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, count: torch.Tensor | None = None) -> None:
@@ -583,7 +561,6 @@ class HipDevice:
                     n_select: int | None = None, workspace: torch.Tensor | None = None):
         """logits [requests * n_beams, vocab] (rows may be apart), scores (float32) and finished (bool) per row. Returns the best
         n_select (default n_beams) continuations of every request as flat (scores, tokens, parents), best first."""
-        self._may_allocate()
         return self._front.beam_select(self.ordinal, logits, scores, n_beams, finished, end_token, n_select, workspace)
 
     def beam_select_workspace(self, n_batch: int, n_beams: int, vocab: int, n_select: int) -> int:
@@ -594,7 +571,6 @@ class HipDevice:
                      tokens: torch.Tensor, end_token: int = 2):
         """The histories [rows, width] after a selection: row i is parents[i]'s with tokens[i] behind it. Returns (history, lens,
         finished)."""
-        self._may_allocate()
         return self._front.beam_advance(self.ordinal, history, lens, finished, parents, tokens, end_token)
 
     # -- tuning hooks -------------------------------------------------------------------

@@ -4,6 +4,8 @@
 // Why native: the kernels behind a decode step take 3 to 10 us, and a call with the same checks in Python over ctypes took 9 to
 // 12 us of the host.  It takes 4 to 5 here: the launch 3.1, torch's allocator 0.8, the rest for some twenty checks.
 #include <ATen/ops/empty.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
@@ -65,6 +67,23 @@ struct Args {
         const double x = PyFloat_AsDouble(v[i]);
         if (x == -1.0 && PyErr_Occurred()) fail(PyExc_TypeError, "%s must be a number", name);
         return x;
+    }
+    // TL_ROTARY_HALF or TL_ROTARY_INTERLEAVED.
+    int layout(int i) const {
+        if (PyUnicode_Check(v[i])) {
+            if (PyUnicode_CompareWithASCIIString(v[i], "half") == 0) return TL_ROTARY_HALF;
+            if (PyUnicode_CompareWithASCIIString(v[i], "interleaved") == 0) return TL_ROTARY_INTERLEAVED;
+        }
+        PyErr_Format(PyExc_ValueError, "unknown layout %R, one of 'half', 'interleaved'", v[i]);
+        throw python_error();
+    }
+    // Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current stream: the
+    // library must enqueue on that one, and launch on this device.
+    void may_allocate() const {
+        const int64_t current = c10::hip::current_device();
+        if (current != ordinal) fail(g_error, "the current device is cuda:%lld, this device is cuda:%lld", (long long)current, (long long)ordinal);
+        if (tl_get_stream() != (void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)ordinal).stream())
+            fail(g_error, "the library stream is not torch's current stream; call bind_stream(torch.cuda.current_stream()) first");
     }
     // A tensor of this device with the given type and number of dimensions.
     const at::Tensor& tensor(int i, const char* name, at::ScalarType type, int64_t dims) const {
@@ -181,10 +200,11 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor& x = a.head_rows(1, "x", -1, -1, -1);
     const int64_t rows = x.size(0), h = x.size(1), d = x.size(2);
     const at::Tensor &positions = a.vector(2, "positions", at::kInt, rows), &freq = a.dense(3, "freq", at::kDouble, 1);
+    a.may_allocate();
     const at::Tensor out = a.none(6) ? at::empty({rows, h, d}, x.options()) : a.head_rows(6, "out", rows, h, d);
     call("tl_rotary_f16", tl_rotary_f16, out.data_ptr(), (size_t)out.stride(0), x.data_ptr(), (size_t)x.stride(0), ptr<int>(positions),
          ptr<double>(freq),
-         size32(2 * freq.numel(), "freq"), a.int32(4, "layout"), (float)a.number(5, "magnitude"), size32(rows, "x"), size32(h, "x"), size32(d, "x"));
+         size32(2 * freq.numel(), "freq"), a.layout(4), (float)a.number(5, "magnitude"), size32(rows, "x"), size32(h, "x"), size32(d, "x"));
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -201,11 +221,12 @@ PyObject* rotary_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor &positions = a.vector(4, "positions", at::kInt, rows), &freq = a.dense(6, "freq", at::kDouble, 1);
     const at::Tensor& tables = a.dense(9, "tables", at::kInt, 2);
     const int* seq_ids = a.none(5) ? nullptr : ptr<int>(a.vector(5, "seq_ids", at::kInt, rows));
+    a.may_allocate();
     const at::Tensor out = a.none(12) ? at::empty({rows, h, cache.head_dim}, q.options()) : a.head_rows(12, "q_out", rows, h, cache.head_dim);
     if (!out.is_contiguous()) fail(PyExc_ValueError, "q_out must be contiguous");
     call("tl_rotary_kv_pages_f16", tl_rotary_kv_pages_f16, out.data_ptr(), q.data_ptr(), (size_t)q.stride(0), k.data_ptr(), (size_t)k.stride(0),
          v.data_ptr(), (size_t)v.stride(0), ptr<int>(positions), seq_ids,
-         ptr<double>(freq), size32(2 * freq.numel(), "freq"), a.int32(10, "layout"), (float)a.number(11, "magnitude"), size32(rows, "q"),
+         ptr<double>(freq), size32(2 * freq.numel(), "freq"), a.layout(10), (float)a.number(11, "magnitude"), size32(rows, "q"),
          size32(h, "q"), &cache, ptr<int>(tables), (size_t)tables.size(1), size32(tables.size(0), "tables"));
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -226,6 +247,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (a.none(7)) max_len = (int)std::min<int64_t>(width * cache.page_size, INT32_MAX);
     else if ((max_len = a.int32(7, "max_len")) < 0) fail(PyExc_ValueError, "max_len %d is out of range", max_len);
     const float scale = a.none(6) ? 1.0f / std::sqrt((float)cache.head_dim) : (float)a.number(6, "scale");
+    a.may_allocate();
     const at::Tensor out = a.none(8) ? at::empty({b, h, cache.head_dim}, q.options()) : a.head_rows(8, "out", b, h, cache.head_dim);
     if (!out.is_contiguous()) fail(PyExc_ValueError, "out must be contiguous");
     const Workspace ws(a, 9, a.none(9) ? tl_paged_attention_workspace(seqs, h, cache.n_kv_heads, cache.head_dim, max_len) : 0, q);
@@ -251,6 +273,7 @@ PyObject* pages_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Args a(args, n, 6, "pages_fork");
     const PageState s(a, 1);
     const at::Tensor& parents = a.vector(4, "parents", at::kInt, s.rows);
+    a.may_allocate();
     Results r(s.tables, {(int64_t)s.rows * s.width, s.rows, s.pages, s.rows, s.rows, 1});
     const at::Tensor tables = r.part({s.rows, s.width}), lens = r.part({s.rows}), refs = r.part({s.pages}), src = r.part({s.rows}), dst =
              r.part({s.rows}), missing = r.part({1});
@@ -267,6 +290,7 @@ PyObject* pages_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Args a(args, n, 6, "pages_extend");
     const PageState s(a, 1);
     const at::Tensor& add = a.vector(4, "add", at::kInt, s.rows);
+    a.may_allocate();
     const at::Tensor missing = at::empty({1}, s.lens.options());
     call("tl_pages_extend", tl_pages_extend, ptr<int>(s.tables), ptr<int>(s.lens), ptr<int>(s.refs), ptr<int>(add), ptr<int>(missing), s.rows,
          s.width, s.pages, a.int32(5, "page_size"));
@@ -292,6 +316,7 @@ PyObject* pages_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Args a(args, n, 3, "pages_compact");
     const at::Tensor &tables = a.dense(1, "tables", at::kInt, 2), &refs = a.dense(2, "refs", at::kInt, 1);
     const int rows = size32(tables.size(0), "tables"), width = size32(tables.size(1), "tables"), pages = size32(refs.size(0), "refs");
+    a.may_allocate();
     Results r(tables, {(int64_t)rows * width, pages, pages, pages, pages, 1});
     const at::Tensor new_tables = r.part({rows, width}), new_refs = r.part({pages}), remap = r.part({pages}), src = r.part({pages});
     const at::Tensor dst = r.part({pages}), count = r.part({1});
@@ -336,6 +361,7 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const uint8_t* finished = a.none(4) ? nullptr : ptr<uint8_t>(a.vector(4, "finished", at::kBool, rows));
     const int batch = size32(rows / beams, "logits"), best = a.none(6) ? beams : a.int32(6, "n_select");
     const int64_t results = best > 0 ? (int64_t)batch * best : 0;
+    a.may_allocate();
     Results r(scores, {results, results, results});
     const at::Tensor new_scores = r.part({results}, at::kFloat), tokens = r.part({results}), parents = r.part({results});
     const Workspace ws(a, 7, a.none(7) ? tl_beam_select_workspace(batch, beams, vocab, best) : 0, scores);
@@ -355,6 +381,7 @@ PyObject* beam_advance(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const uint8_t* finished = a.none(3) ? nullptr : ptr<uint8_t>(a.vector(3, "finished", at::kBool, rows));
     const int out = size32(parents.size(0), "parents");
     const at::Tensor& tokens = a.vector(5, "tokens", at::kInt, out);
+    a.may_allocate();
     Results r(history, {(int64_t)out * width, out, out});
     const at::Tensor new_history = r.part({out, width}), new_lens = r.part({out}), new_finished = r.part({out}, at::kBool);
     call("tl_beam_advance", tl_beam_advance, ptr<int>(new_history), ptr<int>(new_lens), ptr<uint8_t>(new_finished), ptr<int>(history), ptr<int>(lens),

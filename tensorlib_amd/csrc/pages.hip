@@ -97,13 +97,14 @@ struct PageRange {
         return rank;
     }
     // How many pages f picks in the whole pool; *before: in the ranges of the wavefronts before this one.  In the same meeting
-    // the sum of a number `own` of each wavefront, *all_own, and its part before this one, *own_before.
-    template <class F>
-    __device__ int count(F f, int* before, int own, int* own_before, int* all_own) const {
+    // the sum of another number of each wavefront, own(pages picked here): *all_own, and its part before this one, *own_before.
+    template <class F, class G>
+    __device__ int count(F f, int* before, G own, int* own_before, int* all_own) const {
         __shared__ int2 s_count[kWaves];
         const int n = visit(0, 0x7fffffff, f, [](int, int, int) {});
+        const int also = own(n);
         __syncthreads();
-        if (threadIdx.x % 64 == 0) s_count[threadIdx.x / 64] = {n, own};
+        if (threadIdx.x % 64 == 0) s_count[threadIdx.x / 64] = {n, also};
         __syncthreads();
         int all = 0;
         *before = *own_before = *all_own = 0;
@@ -118,11 +119,6 @@ struct PageRange {
             *all_own += c.y;
         }
         return all;
-    }
-    template <class F>
-    __device__ int count(F f, int* before) const {
-        int own_before, all_own;
-        return count(f, before, 0, &own_before, &all_own);
     }
 };
 __device__ __forceinline__ bool is_free(int, int count) { return count == 0; }
@@ -191,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) pages_fork_small_kernel(ForkArgs A) 
     const unsigned long long wanting = __ballot(wants);
     int wanted, before, rank;
     const PageRange range(s_refs, A.n_pages);
-    const int available = range.count(is_free, &before, __popcll(wanting), &rank, &wanted);
+    const int available = range.count(is_free, &before, [&](int) { return (int)__popcll(wanting); }, &rank, &wanted);
     rank += __popcll(wanting & ((1ull << (r % 64)) - 1));
     const bool enough = available >= wanted;
     if (enough) range.visit(before, wanted, is_free, [&](int k, int page, int) {
@@ -277,10 +273,9 @@ __global__ void __launch_bounds__(kThreads) pages_fork_take_kernel(ForkArgs A) {
         wanted += total;
     }
     const PageRange range(A.refs_out, A.n_pages);
-    int before = 0;
-    const int available = wanted ? range.count(is_free, &before) : 0;
+    int before, unused, none;
+    const int available = range.count(is_free, &before, [](int) { return 0; }, &unused, &none);
     if (threadIdx.x == 0) *A.missing = available < wanted ? wanted - available : 0;
-    __syncthreads();
     if (available < wanted) {
         for (int i = threadIdx.x; i < A.n_pages; i += kThreads) A.refs_out[i] = A.refs[i];
         for (size_t i = threadIdx.x; i < (size_t)A.n_seqs * A.table_stride; i += kThreads) A.tables_out[i] = A.tables[i];
@@ -337,7 +332,7 @@ pages_extend_kernel(int* tables, int* lens, int* refs, const int* add, int* miss
         own += __shfl(x, 63, 64);
     }
     int before, own_before, wanted;
-    const int available = range.count(is_free, &before, own, &own_before, &wanted);
+    const int available = range.count(is_free, &before, [&](int) { return own; }, &own_before, &wanted);
     if (refused) s_refused = 1;
     for (int i = 0; i < steps; ++i)
         if (r0 + i * 64 < n_seqs) s_first[r0 + i * 64] += own_before;
@@ -384,37 +379,53 @@ pages_free_kernel(int* tables, int* lens, int* refs, const uint8_t* rows, int ta
     if (threadIdx.x == 0) lens[row] = 0;
 }
 
-// One workgroup: the live pages above the number of live pages move into the free ones below it, in page order.
-__global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(const int* refs, int* copy_src, int* copy_dst, int* count, int n_pages) {
-    const PageRange range(refs, n_pages);
-    int before, holes_before;
-    const int live = range.count([](int, int ref) { return ref > 0; }, &before);
+// New ids and counts, and the rest of the lists, for pages i, i + step, ..  The lists are in page order, so the first mover and
+// the last hole tell a page's part: live and not below the first mover, it moves; free and not above the last hole, it is filled.
+struct CompactArgs {
+    const int* refs;
+    int *refs_out, *remap, *copy_src, *copy_dst, *count;
+    int n_pages;
+};
+__device__ __forceinline__ void compact_apply(const CompactArgs& A, int movers, size_t i, size_t step) {
+    const int first = movers ? A.copy_src[0] : A.n_pages, last = movers ? A.copy_dst[movers - 1] : -1;
+    for (; i < (size_t)A.n_pages; i += step) {
+        const int p = (int)i, ref = A.refs[p];
+        if (ref <= 0) A.remap[p] = -1;
+        else if (p < first) A.remap[p] = p;
+        if (p < first && ref > 0) A.refs_out[p] = ref;
+        else if (p > last || ref > 0) A.refs_out[p] = 0;
+        if (p < movers) {
+            const int from = A.copy_src[p], to = A.copy_dst[p];
+            A.remap[from] = to;
+            A.refs_out[to] = A.refs[from];
+        } else {
+            A.copy_src[p] = A.copy_dst[p] = -1;
+        }
+    }
+}
+__global__ void __launch_bounds__(256) pages_compact_apply_kernel(CompactArgs A) {
+    compact_apply(A, *A.count, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
+}
+// One workgroup: the live pages above the number of live pages move into the free ones below it, in page order.  WHOLE: and all
+// the rest for a pool that one workgroup is soon through with (1000 pages 5.6 against 6.9 us and a launch, 4096 7.9 against 8.2,
+// 8192 11.4 against 10.3).
+constexpr int kWholePages = 4096;
+template <bool WHOLE>
+__global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(CompactArgs A) {
+    const PageRange range(A.refs, A.n_pages);
+    int before, mine = 0, holes_before, unused;
+    const int live = range.count([](int, int ref) { return ref > 0; }, &before, [&](int n) { return mine = n; }, &holes_before, &unused);
     auto mover = [live](int p, int ref) { return ref > 0 && p >= live; };
     auto hole = [live](int p, int ref) { return ref <= 0 && p < live; };
-    const int movers = range.count(mover, &before);
-    range.count(hole, &holes_before);
-    range.visit(before, 0x7fffffff, mover, [&](int k, int p, int) { copy_src[k] = p; });
-    range.visit(holes_before, 0x7fffffff, hole, [&](int k, int p, int) { copy_dst[k] = p; });
-    if (threadIdx.x == 0) *count = movers;
-}
-// New ids and counts, and the rest of the lists.  The lists are in page order, so the first mover and the last hole tell a
-// page's part: live and not below the first mover, it moves; free and not above the last hole, it is filled.
-__global__ void __launch_bounds__(256)
-pages_compact_apply_kernel(const int* refs, int* refs_out, int* remap, int* copy_src, int* copy_dst, const int* count, int n_pages) {
-    const int movers = *count;
-    const int first = movers ? copy_src[0] : n_pages, last = movers ? copy_dst[movers - 1] : -1;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)n_pages; i += (size_t)gridDim.x * 256) {
-        const int p = (int)i, ref = refs[p];
-        if (ref <= 0) remap[p] = -1;
-        else if (p < first) remap[p] = p;
-        if (p < first && ref > 0) refs_out[p] = ref;
-        else if (p > last || ref > 0) refs_out[p] = 0;
-        if (p < movers) {
-            remap[copy_src[p]] = copy_dst[p];
-            refs_out[copy_dst[p]] = refs[copy_src[p]];
-        } else {
-            copy_src[p] = copy_dst[p] = -1;
-        }
+    // of the range's pages below `live`, those that are not live
+    const int below = live < range.begin ? 0 : (live < range.end ? live : range.end) - range.begin;
+    const int movers = range.count(mover, &before, [&](int n) { return below - (mine - n); }, &holes_before, &unused);
+    range.visit(before, 0x7fffffff, mover, [&](int k, int p, int) { A.copy_src[k] = p; });
+    range.visit(holes_before, 0x7fffffff, hole, [&](int k, int p, int) { A.copy_dst[k] = p; });
+    if (threadIdx.x == 0) *A.count = movers;
+    if constexpr (WHOLE) {
+        __syncthreads();
+        compact_apply(A, movers, threadIdx.x, kThreads);
     }
 }
 
@@ -425,36 +436,36 @@ __global__ void __launch_bounds__(256) pages_remap_kernel(int* out, const int* i
     }
 }
 
-// Piece `i` of all pieces of all planes of all pairs: 256 threads x 4 x 16 bytes.  STREAM: accesses that do not settle in the
-// caches, for calls that may move more than fits there.
-constexpr unsigned kPiece = 256 * 4 * 16;
+// A piece is 256 threads x 4 x 16 bytes of a pair's page in all planes, one plane's after the other's: pages may be much
+// smaller than a piece (16 planes of 1 KB, 1100 pairs: 29 -> 15 us with the numbering).  STREAM: accesses that do not settle in the caches, for calls that may move more than fits there.
+constexpr unsigned kPiece = 256 * 4;       // in units of 16 bytes
 template <bool STREAM>
 __global__ void __launch_bounds__(256)
-pages_copy_kernel(unsigned char* pool, size_t plane_stride, size_t page_stride, size_t page_bytes, unsigned pieces, int n_planes, int n_pages,
-                  const int* src, const int* dst, const int* count, int max_pairs) {
-    int pairs = max_pairs;
-    if (count) pairs = min(max(*count, 0), max_pairs);
-    const size_t per_pair = (size_t)pieces * n_planes, total = per_pair * pairs;
-    for (size_t i = blockIdx.x; i < total; i += gridDim.x) {
-        const size_t pair = i / per_pair, rest = i % per_pair;
+pages_copy_kernel(unsigned char* pool, size_t plane_stride, size_t page_stride, FastDiv by_page, FastDiv by_pieces, unsigned units, int n_pages, const int* src,
+                  const int* dst, const int* count, int max_pairs) {
+    const unsigned pairs = count ? (unsigned)min(max(*count, 0), max_pairs) : (unsigned)max_pairs;
+    unsigned piece, step;
+    unsigned pair = by_pieces.divmod(blockIdx.x, piece);
+    const unsigned pair_step = by_pieces.divmod(gridDim.x, step);
+    for (; pair < pairs; pair += pair_step + (piece + step >= by_pieces.d), piece = piece + step >= by_pieces.d ? piece + step - by_pieces.d : piece + step) {
+        const unsigned first = piece * kPiece + threadIdx.x;
         const int from = src[pair], to = dst[pair];
         if (from < 0 || from >= n_pages || to < 0 || to >= n_pages) continue;
-        const size_t plane = rest / pieces, at = (rest % pieces) * kPiece;
-        const unsigned char* s = pool + plane * plane_stride + from * page_stride + at;
-        unsigned char* d = pool + plane * plane_stride + to * page_stride + at;
-        const size_t left = page_bytes - at;
         float4_t x[4];
+        size_t at[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const unsigned o = (j * 256 + threadIdx.x) * 16;
-            const float4_t* from4 = reinterpret_cast<const float4_t*>(s + o);
-            if (o < left) x[j] = STREAM ? __builtin_nontemporal_load(from4) : *from4;
+            const unsigned u = first + j * 256;
+            unsigned unit;
+            const unsigned plane = by_page.divmod(u, unit);
+            at[j] = plane * plane_stride + (size_t)unit * 16;
+            const float4_t* from4 = reinterpret_cast<const float4_t*>(pool + from * page_stride + at[j]);
+            if (u < units) x[j] = STREAM ? __builtin_nontemporal_load(from4) : *from4;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const unsigned o = (j * 256 + threadIdx.x) * 16;
-            float4_t* to4 = reinterpret_cast<float4_t*>(d + o);
-            if (o >= left) continue;
+            float4_t* to4 = reinterpret_cast<float4_t*>(pool + to * page_stride + at[j]);
+            if (first + j * 256 >= units) continue;
             if (STREAM) __builtin_nontemporal_store(x[j], to4);
             else *to4 = x[j];
         }
@@ -546,10 +557,16 @@ int tl_pages_compact(const int* tables, const int* refs, int* tables_out, int* r
     TL_REQUIRE(refs && refs_out && remap && copy_src && copy_dst && count && (n_seqs == 0 || (tables && tables_out)), "%s: null pointer", what);
     TL_REQUIRE(refs_out != refs, "%s: the new reference counts must not lie over the old ones", what);
     TL_ENSURE_INIT();
-    pages_compact_plan_kernel<<<1, kThreads, 0, stream()>>>(refs, copy_src, copy_dst, count, n_pages);
-    TL_CHECK_LAUNCH("pages_compact_plan_kernel");
-    pages_compact_apply_kernel<<<ints_grid(n_pages), 256, 0, stream()>>>(refs, refs_out, remap, copy_src, copy_dst, count, n_pages);
-    TL_CHECK_LAUNCH("pages_compact_apply_kernel");
+    const CompactArgs A{refs, refs_out, remap, copy_src, copy_dst, count, n_pages};
+    if (n_pages <= kWholePages) {
+        pages_compact_plan_kernel<true><<<1, kThreads, 0, stream()>>>(A);
+        TL_CHECK_LAUNCH("pages_compact_plan_kernel");
+    } else {
+        pages_compact_plan_kernel<false><<<1, kThreads, 0, stream()>>>(A);
+        TL_CHECK_LAUNCH("pages_compact_plan_kernel");
+        pages_compact_apply_kernel<<<ints_grid(n_pages), 256, 0, stream()>>>(A);
+        TL_CHECK_LAUNCH("pages_compact_apply_kernel");
+    }
     const size_t n = (size_t)n_seqs * table_stride;
     if (n > 0) {
         pages_remap_kernel<<<ints_grid(n), 256, 0, stream()>>>(tables_out, tables, remap, n_pages, n);
@@ -568,19 +585,20 @@ int tl_pages_copy(void* pool, size_t plane_stride, size_t page_stride, size_t pa
     TL_REQUIRE(aligned16(pool) && plane_stride % 16 == 0 && page_stride % 16 == 0 && page_bytes % 16 == 0,
                "%s: the pool, its strides and the page size must be multiples of 16 bytes", what);
     TL_REQUIRE(page_stride >= page_bytes || n_pages == 1, "%s: pages overlap", what);
-    const size_t pieces = (page_bytes + kPiece - 1) / kPiece;
-    if (pieces > 0x7fffffffu) return set_error(TL_ELIMIT, "%s: pages of %zu bytes are too large", what, page_bytes);
+    const double all_units = (double)page_bytes / 16 * n_planes;
+    if (all_units > 2147482624.0) return set_error(TL_ELIMIT, "%s: %d pages of %zu bytes are too much for one pair", what, n_planes, page_bytes);
     TL_ENSURE_INIT();
+    const unsigned units = (unsigned)(page_bytes / 16 * n_planes), pieces = (units + kPiece - 1) / kPiece;
     // Past the caches from 256 MB of possible moves on (the host knows no more): packing 4096 pages of 16 x 32 KB, of which a
-    // quarter moves, takes 210 us, 5.4 TB/s, against 237; 192 rows of which 48 copy 64 x 8 KB 28 against 29.5 the other way.
+    // quarter moves, takes 206 us, 5.5 TB/s, against 237; 192 rows of which 48 copy 64 x 8 KB 22 against 24 the other way.
     // The workgroups share the possible pieces, about four each: with fewer of them the ones with work become too few.
-    const double total = (double)pieces * n_planes * max_pairs;
-    const bool past = (double)page_bytes * n_planes * max_pairs >= 268435456.0;
+    const double total = (double)pieces * max_pairs;
+    const bool past = all_units * 16 * max_pairs >= 268435456.0;
     double blocks = total / 4 < 4096.0 ? 4096.0 : total / 4 < 24576.0 ? total / 4 : 24576.0;
     if (!past) blocks = 4096.0;
     if (blocks > total) blocks = total;
     auto kernel = past ? pages_copy_kernel<true> : pages_copy_kernel<false>;
-    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(static_cast<unsigned char*>(pool), plane_stride, page_stride, page_bytes, (unsigned)pieces, n_planes,
+    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(static_cast<unsigned char*>(pool), plane_stride, page_stride, FastDiv((unsigned)(page_bytes / 16)), FastDiv(pieces), units,
                                                    n_pages, src, dst, count, max_pairs);
     TL_CHECK_LAUNCH("pages_copy_kernel");
     return TL_OK;

@@ -474,7 +474,7 @@ def test_free(dev):
     assert np.array_equal(r.cpu().numpy(), np.bincount(tables[tables >= 0], minlength=len(refs)))
 
 
-@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (10, 10), (10, 0), (100, 37), (1024, 512), (5000, 4999), (4097, 1), (20000, 9000), (16384, 16383), (16385, 8000), (131072, 70000)])
+@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (10, 10), (10, 0), (100, 37), (1024, 512), (5000, 4999), (4096, 1500), (4097, 1), (20000, 9000), (16384, 16383), (16385, 8000), (131072, 70000)])
 def test_compact(dev, n_pages, live):
     rng = np.random.RandomState(n_pages + live)
     refs = np.zeros(n_pages, np.int64)

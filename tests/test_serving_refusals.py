@@ -124,6 +124,7 @@ def test_attention_limits_and_empty_batch():
     ("tl_pages_copy", COPY, dict(page_bytes=250), "16 bytes", TL_EINVAL), ("tl_pages_copy", COPY, dict(pool=P + 8), "16 bytes", TL_EINVAL),
     ("tl_pages_copy", COPY, dict(plane_stride=4100), "16 bytes", TL_EINVAL), ("tl_pages_copy", COPY, dict(page_stride=128), "overlap", TL_EINVAL),
     ("tl_pages_copy", COPY, dict(max_pairs=-1), "negative", TL_EINVAL),
+    ("tl_pages_copy", COPY, dict(page_bytes=1 << 40, page_stride=1 << 40), "too much", TL_ELIMIT),
     ("tl_beam_select_f16", SELECT, dict(logits=None), "null", TL_EINVAL), ("tl_beam_select_f16", SELECT, dict(scores=None), "null", TL_EINVAL),
     ("tl_beam_select_f16", SELECT, dict(n_select=65), "at most", TL_ELIMIT), ("tl_beam_select_f16", SELECT, dict(n_beams=1025), "at most", TL_ELIMIT),
     ("tl_beam_select_f16", SELECT, dict(n_beams=1, vocab=3), "do not exist", TL_EINVAL), ("tl_beam_select_f16", SELECT, dict(finished=P, end_token=100), "outside", TL_EINVAL),

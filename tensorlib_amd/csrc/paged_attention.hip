@@ -16,9 +16,9 @@
 // layouts that need no exchange at all; its rate made 0.9 us of a 32-position turn: 13.7 against 12.4 us for 1 x 2048
 // positions of 32 heads, 108 against 92 us for 16 x 8000 positions of 256 dims.)
 //
-// Measured (one pass, both launches): 64 sequences of 65 to 4097 positions, 32 heads on 8 of 128: 121 us = 4.6 TB/s; in
+// Measured (one pass, both launches): 64 sequences of 65 to 4097 positions, 32 heads on 8 of 128: 114 us = 4.85 TB/s; in
 // the middle of the launch the memory runs at 6.0, the rest is the first requests' and the last workgroups' time.
-// 4 sequences of 100001 to 131072, 64 heads on 8: 354 us = 5.4 TB/s.  1 x 2048, 32 heads: 12.0 us, of which the two
+// 4 sequences of 100001 to 131072, 64 heads on 8: 320 us = 5.95 TB/s.  1 x 2048, 32 heads: 12.0 us, of which the two
 // launches of an empty problem take 8.
 #include <cmath>
 
@@ -387,14 +387,32 @@ __global__ void __launch_bounds__(THREADS) paged_attention_join_kernel(PagedAttn
     *reinterpret_cast<half4_t*>(A.out + ((size_t)seq * A.n_heads + h) * D + d) = r;
 }
 
-// Positions per workgroup.  512: a workgroup then lives for 20 us in a saturated memory system, and the last ones of a
-// ragged batch end close together (64 sequences of 65 to 4097 positions, 32 heads on 8: 121 us, against 134 with 2048 and
-// 132 with 128).  1024 for long contexts, where the partials are what can be saved (4 x 131072: 352 against 362 us).
-// Fewer as long as there are not four workgroups per compute unit (1 x 32768: 38 us with 256, 40 with 128, 47 with 1024).
-static int chunk_of(int n_seqs, int head_tiles, int max_len) {
-    int chunk = max_len > 32768 ? kMaxChunk : kMaxChunk / 2;
-    while (chunk > kMinChunk && (double)n_seqs * head_tiles * ((max_len + (double)chunk - 1) / chunk) < 1024.0) chunk /= 2;
-    return chunk;
+// Positions per workgroup.  With fewer workgroups than six times the 256 compute units, the least of: positions that the fullest
+// unit goes through one after the other, 42 more for each workgroup it is given, 240 for the join (in units of 128 dims, fitted
+// to thirty sizes).  It cuts 1 x 4096 on 8 kv heads into chunks of 128 (10.2 us, 13.7 with 512), 1 x 131072 on one into 512
+// (20.5, 28.2 with 128), 2 x 60000 on 2 into 1024 (29.5, 37 with 128), and leaves 64 x 700 on 8 whole (29.5, 42 with 512).  With
+// more: 512, since the last workgroups of a ragged batch then end close together (64 of 65 to 4097 positions on 8: 114 us, 117
+// with 1024, 135 with 128), 1024 for long contexts, where the partials are what can be saved (4 x 131072: 320, 332 with 512),
+// and where it leaves sequences whole (200 x 600: 60, 87 with 512).
+static int chunk_of(int n_seqs, int head_tiles, int head_dim, int max_len) {
+    constexpr double kUnits = 256.0;
+    const double tiles = (double)n_seqs * head_tiles, dims = head_dim <= 64 ? 0.5 : head_dim <= 128 ? 1.0 : 2.0;
+    int best = kMaxChunk;
+    if (tiles * ceil(max_len / 512.0) * dims >= 6 * kUnits) {
+        if (max_len > kMaxChunk && max_len <= 32768) best = kMaxChunk / 2;
+    } else {
+        double least = 1e300;
+        for (int chunk = kMaxChunk; chunk >= kMinChunk; chunk /= 2) {
+            const double groups = tiles * ceil((double)max_len / chunk);
+            const double time = ceil(groups / kUnits) * (chunk < max_len ? chunk : max_len) * dims + 42.0 * groups / kUnits + (chunk < max_len ? 240.0 : 0.0);
+            if (time < least) {
+                best = chunk;
+                least = time;
+            }
+        }
+    }
+    while (best > kMinChunk && best / 2 >= max_len) best /= 2;
+    return best;
 }
 static int group_tiles_of(int n_heads, int n_kv_heads) { return (n_heads / n_kv_heads + kGroupTile - 1) / kGroupTile; }
 
@@ -412,7 +430,7 @@ extern "C" {
 
 size_t tl_paged_attention_workspace(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len) {
     if (n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || head_dim <= 0 || max_len <= 0) return 0;
-    const int chunk = tl::chunk_of(n_seqs, n_kv_heads * tl::group_tiles_of(n_heads, n_kv_heads), max_len);
+    const int chunk = tl::chunk_of(n_seqs, n_kv_heads * tl::group_tiles_of(n_heads, n_kv_heads), head_dim, max_len);
     const size_t splits = ((size_t)max_len + chunk - 1) / chunk;
     return splits <= 1 ? 0 : splits * n_seqs * n_heads * ((size_t)head_dim + 2) * sizeof(float);
 }
@@ -435,7 +453,7 @@ int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_k
     A.group = n_heads / cache->n_kv_heads;
     A.group_tiles = group_tiles_of(n_heads, cache->n_kv_heads);
     const int head_tiles = cache->n_kv_heads * A.group_tiles;
-    A.chunk = chunk_of(n_seqs, head_tiles, max_len);
+    A.chunk = chunk_of(n_seqs, head_tiles, cache->head_dim, max_len);
     A.n_splits = max_len <= A.chunk ? 1 : (int)(((size_t)max_len + A.chunk - 1) / A.chunk);
     const size_t parts = (size_t)n_seqs * A.n_splits * n_heads;
     if (A.n_splits > 1) {

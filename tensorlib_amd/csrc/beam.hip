@@ -116,11 +116,12 @@ __device__ __forceinline__ T smallest_group_maximum(T v, int groups_log2) {
     return over_wave(v, [groups_log2](T a, T b, int bit) { return (bit < 6 - groups_log2) == (b > a) ? b : a; });
 }
 
-// The n-th largest of the wavefront's keys, bit by bit from the top.
+// The n-th largest of the wavefront's keys without its lowest 12 bits, bit by bit from the top: of a float's place eleven bits
+// of the fraction are left, close enough for a bound, and 0.25 us less than with all 32 in turn.
 __device__ __forceinline__ unsigned nth_largest(unsigned key, int n) {
     unsigned found = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int bit = 31; bit >= 12; --bit) {
         const unsigned trial = found | (1u << bit);
         if ((int)__popcll(__ballot(key >= trial)) >= n) found = trial;
     }
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
     const unsigned bound = nth_largest(order_of(low), A.n_select);
     if (lane == 0) s_bound[wave] = bound;
     __syncthreads();
-    const double reach = (double)from_order(wave_max(s_bound[lane % kPickWaves]));
+    const double reach = (double)from_order(max(wave_max(s_bound[lane % kPickWaves]), order_of(-INFINITY)));
     auto list = [&](const Choice& c) {
         if (c.place == none || !(c.score >= reach)) return;
         const int at = atomicAdd(&s_count, 1);

@@ -462,7 +462,8 @@ int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_k
         TL_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", what);
     }
     const double blocks = (double)n_seqs * A.n_splits * head_tiles;
-    if (blocks >= 2147483648.0 || n_seqs > 65535) return set_error(TL_ELIMIT, "%s: %d sequences of up to %d positions are too many for one call", what, n_seqs, max_len);
+    // threads of one dimension of a grid are counted in 32 bits
+    if (blocks >= 16777216.0 || (A.n_splits > 1 && n_heads >= 4194304) || n_seqs > 65535) return set_error(TL_ELIMIT, "%s: %d sequences of up to %d positions are too many for one call", what, n_seqs, max_len);
     TL_ENSURE_INIT();
     A.out = static_cast<half_t*>(out);
     A.q = static_cast<const half_t*>(q);

@@ -174,14 +174,16 @@ constexpr double kStreamValues = 4194304.0;
 
 static int launch_rotary(RotaryArgs& A, int n_tokens, int layout, bool vectors, const char* what) {
     const bool half = layout == TL_ROTARY_HALF;
-    const int n_rows = A.n_heads + 2 * A.n_kv;
+    const long n_rows = A.n_heads + 2L * A.n_kv;
     vectors = vectors && A.head_dim % 8 == 0 && A.rotary_dim % (half ? 16 : 8) == 0;
-    const int units = vectors ? (half ? A.head_dim / 8 - A.rotary_dim / 16 : A.head_dim / 8) : (A.head_dim + 1) / 2;
+    const int units = vectors ? (half ? A.head_dim / 8 - A.rotary_dim / 16 : A.head_dim / 8) : (int)((A.head_dim + 1L) / 2);
     const bool stream_ = vectors && (double)n_tokens * n_rows * A.head_dim >= kStreamValues;
     const int rows = stream_ ? 2 : 1;
-    const int groups = (n_rows + rows - 1) / rows;
+    const long groups = (n_rows + rows - 1) / rows;
     const double total = (double)n_tokens * groups * units;
-    if (total >= 2147483648.0) return set_error(TL_ELIMIT, "%s: %d tokens of %d heads of %d are too many for one call", what, n_tokens, n_rows, A.head_dim);
+    if (total >= 2147483648.0 || n_rows > 0x7fffffff)
+        return set_error(TL_ELIMIT, "%s: %d tokens of %ld heads of %d are too many for one call", what, n_tokens, n_rows, A.head_dim);
+    TL_ENSURE_INIT();
     A.total = (unsigned)total;
     A.by_units = FastDiv((unsigned)units);
     A.by_groups = FastDiv((unsigned)groups);
@@ -252,7 +254,6 @@ int tl_rotary_f16(void* out, size_t out_stride, const void* in, size_t in_stride
     const size_t width = (size_t)n_heads * head_dim;
     TL_REQUIRE(n_tokens == 1 || (in_stride >= width && out_stride >= width), "tl_rotary_f16: row strides must cover the heads");
     TL_REQUIRE(out != in || out_stride == in_stride || n_tokens == 1, "tl_rotary_f16: in place needs equal strides");
-    TL_ENSURE_INIT();
     RotaryArgs A{};
     A.q_out = static_cast<half_t*>(out);
     A.q = static_cast<const half_t*>(in);
@@ -286,7 +287,6 @@ int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const vo
     if (n_tokens > 1)
         TL_REQUIRE(q_stride >= n_heads * D && k_stride >= cache->n_kv_heads * D && v_stride >= cache->n_kv_heads * D,
                    "%s: row strides must cover the heads", what);
-    TL_ENSURE_INIT();
     RotaryArgs A{};
     A.q_out = static_cast<half_t*>(q_out);
     A.q = static_cast<const half_t*>(q);

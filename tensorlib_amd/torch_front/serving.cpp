@@ -77,11 +77,15 @@ struct Args {
         PyErr_Format(PyExc_ValueError, "unknown layout %R, one of 'half', 'interleaved'", v[i]);
         throw python_error();
     }
-    // Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current stream: the
-    // library must enqueue on that one, and launch on this device.
-    void may_allocate() const {
+    // The library launches on the current device.
+    void on_device() const {
         const int64_t current = c10::hip::current_device();
         if (current != ordinal) fail(g_error, "the current device is cuda:%lld, this device is cuda:%lld", (long long)current, (long long)ordinal);
+    }
+    // Results and workspaces come from torch's allocator, which hands memory out in the order of torch's current stream: the
+    // library must enqueue on that one.
+    void may_allocate() const {
+        on_device();
         if (tl_get_stream() != (void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)ordinal).stream())
             fail(g_error, "the library stream is not torch's current stream; call bind_stream(torch.cuda.current_stream()) first");
     }
@@ -304,6 +308,7 @@ PyObject* pages_free(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Args a(args, n, 6, "pages_free");
     const PageState s(a, 1);
     const at::Tensor& rows = a.vector(4, "rows", at::kBool, s.rows);
+    a.on_device();
     call("tl_pages_free", tl_pages_free, ptr<int>(s.tables), ptr<int>(s.lens), ptr<int>(s.refs), ptr<uint8_t>(rows), s.rows, s.width, s.pages,
          a.int32(5, "page_size"));
     Py_RETURN_NONE;
@@ -341,6 +346,7 @@ PyObject* pages_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor& src = a.dense(2, "src", at::kInt, 1);
     const at::Tensor& dst = a.vector(3, "dst", at::kInt, src.size(0));
     const int* count = a.none(4) ? nullptr : ptr<int>(a.vector(4, "count", at::kInt, 1));
+    a.on_device();
     call("tl_pages_copy", tl_pages_copy, pool.data_ptr(), (size_t)(pool.stride(0) * item), (size_t)(pool.stride(1) * item), (size_t)page_bytes,
          size32(pool.size(0), "pool"), size32(pool.size(1), "pool"), ptr<int>(src), ptr<int>(dst), count, size32(src.size(0), "src"));
     Py_RETURN_NONE;

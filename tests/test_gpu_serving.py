@@ -902,3 +902,23 @@ def test_calls_from_several_threads(dev):
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+def test_the_current_device_and_stream_are_checked(dev):
+    """What allocates runs on torch's current stream only; what does not may run on the library's own."""
+    pool = rand((2, 6, 16), 1)
+    want = pool.clone()
+    want[:, 3] = pool[:, 5]
+    tables, lens, refs = ints([[0, 1]]), ints([7]), ints([1, 1, 0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    dev.bind_stream(side)
+    try:
+        for call in (lambda: dev.pages_extend(tables, lens, refs, ints([1]), 4), lambda: dev.rotary(rand((1, 1, 8), 2), ints([0]), dev.rotary_frequencies(8))):
+            with pytest.raises(TensorLibError, match="stream"):
+                call()
+        dev.pages_copy(pool, ints([5]), ints([3]))
+        torch.cuda.synchronize()
+        assert torch.equal(pool, want) and lens.tolist() == [7]
+    finally:
+        dev.bind_stream(torch.cuda.current_stream())

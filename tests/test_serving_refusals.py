@@ -63,6 +63,16 @@ def test_rotary_refuses(kw, match):
     refused("tl_rotary_f16", changed(ROTARY, **kw), match)
 
 
+def test_sizes_past_a_launch_are_refused():
+    many = dict(n_tokens=1 << 20, n_heads=1 << 12, in_stride=1 << 18, out_stride=1 << 18)
+    refused("tl_rotary_f16", changed(ROTARY, **many), "too many", TL_ELIMIT)
+    refused("tl_rotary_f16", changed(ROTARY, n_tokens=1, n_heads=2 ** 31 - 1), "too many", TL_ELIMIT)
+    refused("tl_rotary_kv_pages_f16", changed(ROTARY_PAGED, n_tokens=1, n_heads=1, rotary_dim=0, cache=cache(n_kv_heads=2 ** 31 - 1, head_dim=8)), "too many",
+            TL_ELIMIT)
+    args = changed(ATTENTION, cache=cache(), n_seqs=65535, max_len=200000, ws=P, ws_bytes=1 << 40)
+    refused("tl_paged_attention_f16", args, "too many", TL_ELIMIT)
+
+
 def test_rotary_of_no_tokens():
     rc, _ = call("tl_rotary_f16", *changed(ROTARY, n_tokens=0, out=None, x=None, positions=None, freq=None))
     assert rc == 0          # nothing to do is no error

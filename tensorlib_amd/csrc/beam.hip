@@ -10,14 +10,15 @@
 // candidates in order: within a row the order of the logits is the order of the scores, so no sum is needed for that.
 // Second launch: one workgroup per request joins the rows' sums and picks.
 //
-// The best n of many: cut the lanes into G >= n groups; the smallest of the groups' maxima is a bound that at least n elements
-// reach.  The groups may be those of one wavefront, or a share of each wavefront's; the largest such bound is taken.  What reaches it (some twenty candidates for n = 8 out of 8192 random logits) goes to a list in LDS,
-// where every candidate counts those before it: its rank is its place in the answer.  A list that overflows (values in
-// an order that defeats the bound) is given up for n rounds of a maximum over the workgroup.
+// The best n of many: the n-th largest of the threads' maxima, or the least of what each wavefront's share of n threads reaches,
+// is a bound that at least n elements reach; it is found bit by bit, a ballot each.  What reaches it (some fifteen candidates
+// for n = 8 out of 8192 random logits) goes to a list in LDS, where every candidate counts those before it: its rank is its
+// place in the answer.  A list that overflows (values in an order that defeats the bound) is given up for n rounds of a maximum
+// over the workgroup.
 //
-// 24 requests of 8 beams over 100003 tokens: 16 + 6 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
-// for 8 us of the first launch, and its workgroups do not all run at a time).  1 request of 4 beams over 32000: 4 + 4 us,
-// two launches and their memory latencies.
+// 24 requests of 8 beams over 100003 tokens: 13 + 6 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
+// for 7 us of the first launch, and its workgroups do not all run at a time).  1 request of 4 beams over 32000: 4 + 4 us,
+// two launches and their memory latencies.  64 beams over 100003, 64 selected: 120 us, most of it the second launch.
 #include <cmath>
 
 #include "paged.h"
@@ -48,7 +49,7 @@ struct BeamArgs {
     SliceStats* stats;                                    // [row][slice]
     unsigned* best;                                       // [row][slice][n_select]
     FastDiv by_row;                                       // candidates per row in the second launch
-    int n_beams, vocab, n_select, end_token, n_slices, slice, groups_log2;
+    int n_beams, vocab, n_select, end_token, n_slices, slice;
 };
 
 // Larger is better: the logit's order (the two zeros are equal), then the lower index in the slice.  Never 0.
@@ -110,12 +111,6 @@ template <class T>
 __device__ __forceinline__ T wave_sum(T v) {
     return over_wave(v, [](T a, T b, int) { return a + b; });
 }
-// The smallest over 2^groups_log2 groups of adjacent lanes of the group's largest value.
-template <class T>
-__device__ __forceinline__ T smallest_group_maximum(T v, int groups_log2) {
-    return over_wave(v, [groups_log2](T a, T b, int bit) { return (bit < 6 - groups_log2) == (b > a) ? b : a; });
-}
-
 // The n-th largest of the wavefront's keys without its lowest 12 bits, bit by bit from the top: of a float's place eleven bits
 // of the fraction are left, close enough for a bound, and 0.25 us less than with all 32 in turn.
 __device__ __forceinline__ unsigned nth_largest(unsigned key, int n) {
@@ -125,6 +120,26 @@ __device__ __forceinline__ unsigned nth_largest(unsigned key, int n) {
         const unsigned trial = found | (1u << bit);
         if ((int)__popcll(__ballot(key >= trial)) >= n) found = trial;
     }
+    return found;
+}
+// The n-th largest of the wavefront's candidates, or one a little smaller: by the logit, and by the index too where many have
+// that logit (a row that is masked but for a few tokens).
+__device__ __forceinline__ unsigned nth_candidate(unsigned c, int n) {
+    unsigned found = 0;
+    int reached = 64;
+    auto bits = [&](int from, int to) {
+#pragma unroll
+        for (int bit = from; bit >= to; --bit) {
+            const unsigned trial = found | (1u << bit);
+            const int k = (int)__popcll(__ballot(c >= trial));
+            if (k >= n) {
+                found = trial;
+                reached = k;
+            }
+        }
+    };
+    bits(kIndexBits + 15, kIndexBits);
+    if (reached > 2 * n + 4) bits(kIndexBits - 1, 0);
     return found;
 }
 // A float's place in the order of floats, and back.
@@ -147,7 +162,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
     constexpr int SLICE = NV * kBeamThreads * 8;
     static_assert(SLICE <= 1 << kIndexBits, "index bits");
     __shared__ __align__(16) unsigned s_list[kList];
-    __shared__ unsigned s_bound[kBeamWaves], s_share[kBeamWaves], s_best[kBeamWaves];
+    __shared__ unsigned s_bound[kBeamWaves], s_best[kBeamWaves];
     __shared__ float s_c[kBeamWaves];
     __shared__ double s_sum[kBeamWaves];
     __shared__ int s_count;
@@ -200,24 +215,21 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
         if (most[j] == top) first = j;
     // the candidate of the piece's last element is at most the thread's best: still a bound that enough elements reach
     const unsigned mine_least = candidate(top, (first * kBeamThreads + tid) * 8 + 7);
-    const unsigned bound = smallest_group_maximum(mine_least, A.groups_log2);
-    const unsigned share = smallest_group_maximum(mine_least, A.groups_log2 > 2 ? A.groups_log2 - 2 : 0);
+    // Either every wavefront's share of n_select, the least of which n_select threads reach together, or, where the last one has
+    // little to choose from, the best of what n_select threads of one reach.
+    const bool shared = n >= kBeamThreads * 7;
+    const unsigned bound = nth_candidate(mine_least, shared ? (A.n_select + kBeamWaves - 1) / kBeamWaves : A.n_select);
     const float c_wave = wave_max(c_thread);
     const double sum_wave = wave_sum((double)ldexpf(mine_sum, exponent_of(c_thread, c_wave)));
     if (tid % 64 == 0) {
         s_bound[wave] = bound;
-        s_share[wave] = share;
         s_c[wave] = c_wave;
         s_sum[wave] = sum_wave;
     }
     __syncthreads();
-    unsigned reach = 0, all = ~0u;
+    unsigned reach = s_bound[0];
 #pragma unroll
-    for (int w = 0; w < kBeamWaves; ++w) {
-        reach = max(reach, s_bound[w]);
-        all = min(all, s_share[w]);
-    }
-    reach = max(reach, all);
+    for (int w = 1; w < kBeamWaves; ++w) reach = shared ? min(reach, s_bound[w]) : max(reach, s_bound[w]);
     if (tid == 0) {
         float c_slice = kLowest;
         double sum = 0.0;
@@ -250,15 +262,19 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
     unsigned* best = A.best + ((size_t)row * A.n_slices + slice) * A.n_select;
     const int count = s_count;
     if (count <= kList) {
-        for (int i = tid; i < count; i += kBeamThreads) {
+        // several threads count for each candidate where there are enough
+        const int parts = count <= kBeamThreads / 8 ? 8 : count <= kBeamThreads / 4 ? 4 : count <= kBeamThreads / 2 ? 2 : 1;
+        for (int i = tid / parts; i < count; i += kBeamThreads) {      // once if parts > 1: all of a candidate's lanes come along
             const unsigned mine = s_list[i];
             int rank = 0;
-            for (int k = 0; k < count; k += 8) {          // what stands behind the list's end is masked
-                const uint4 a = *reinterpret_cast<const uint4*>(s_list + k), b = *reinterpret_cast<const uint4*>(s_list + k + 4);
+            for (int k = tid % parts * 4; k < count; k += parts * 4) {     // what stands behind the list's end is masked
+                const uint4 a = *reinterpret_cast<const uint4*>(s_list + k);
                 rank += (a.x > mine) + (k + 1 < count && a.y > mine) + (k + 2 < count && a.z > mine) + (k + 3 < count && a.w > mine);
-                rank += (k + 4 < count && b.x > mine) + (k + 5 < count && b.y > mine) + (k + 6 < count && b.z > mine) + (k + 7 < count && b.w > mine);
             }
-            if (rank < A.n_select) best[rank] = mine;
+            if (parts >= 2) rank = join<0>(rank, [](int a, int b) { return a + b; });
+            if (parts >= 4) rank = join<1>(rank, [](int a, int b) { return a + b; });
+            if (parts == 8) rank = join<2>(rank, [](int a, int b) { return a + b; });
+            if (tid % parts == 0 && rank < A.n_select) best[rank] = mine;
         }
         for (int i = count + tid; i < A.n_select; i += kBeamThreads) best[i] = 0;       // the slice has no more
         return;
@@ -292,15 +308,15 @@ struct Choice {
 };
 __device__ __forceinline__ bool better(const Choice& a, const Choice& b) { return a.score > b.score || (a.score == b.score && a.place < b.place); }
 
-constexpr int kPickThreads = 1024;
-constexpr int kPickWaves = kPickThreads / 64;
 constexpr int kHeld = 4;                                  // continuations a thread keeps in registers
 
-__global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) beam_pick_kernel(BeamArgs A) {
+    constexpr int kPickThreads = THREADS, kPickWaves = THREADS / 64;
     __shared__ Choice s_list[kList];
     __shared__ Choice s_best[kPickWaves];
     __shared__ Choice s_last;
-    __shared__ unsigned s_bound[kPickWaves];
+    __shared__ unsigned s_bound[kPickWaves], s_share[kPickWaves];
     __shared__ int s_count;
     extern __shared__ double s_base[];                    // per beam: score - log sum, then how it continues
     int* s_kind = reinterpret_cast<int*>(s_base + A.n_beams);
@@ -359,10 +375,22 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
         if (e == 0) return {-INFINITY, none};
         return {base + (double)candidate_logit(e), (u64)b << 32 | ((at / A.n_select) * A.slice + candidate_index(e))};
     };
-    auto choice = [&](unsigned i) -> Choice {
+    auto entry = [&](unsigned i) -> unsigned {
         unsigned at;
         const int b = (int)A.by_row.divmod(i, at);
-        return choice_of(i, s_kind[b] == kAlive && (int)at < per_row ? A.best[(size_t)(row0 + b) * per_row + at] : 0);
+        return s_kind[b] == kAlive && (int)at < per_row ? A.best[(size_t)(row0 + b) * per_row + at] : 0;
+    };
+    auto choice = [&](unsigned i) -> Choice { return choice_of(i, entry(i)); };
+    // f of the continuations that are not held, several of whose entries are under way together
+    auto others = [&](auto f) {
+        for (unsigned i0 = kHeld * kPickThreads + tid; i0 < total; i0 += 4 * kPickThreads) {
+            unsigned e[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e[x] = i0 + x * kPickThreads < total ? entry(i0 + x * kPickThreads) : 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (i0 + x * kPickThreads < total) f(choice_of(i0 + x * kPickThreads, e[x]));
+        }
     };
     auto put = [&](int k, const Choice& c) {
         const size_t o = (size_t)request * A.n_select + k;
@@ -379,15 +407,22 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
         if (i < total) kept[x] = choice_of(i, held[x]);
         mine = fmax(mine, kept[x].score);
     }
-    for (unsigned i = kHeld * kPickThreads + tid; i < total; i += kPickThreads) mine = fmax(mine, choice(i).score);
+    others([&](const Choice& c) { mine = fmax(mine, c.score); });
     // the n-th largest of a wavefront's threads, as a float that is not above it: scores of one beam in neighbouring threads
     // are in order already, and groups of them would make a loose bound
     float low = (float)mine;
     if ((double)low > mine) low = from_order(order_of(low) - 1);
     const unsigned bound = nth_largest(order_of(low), A.n_select);
-    if (lane == 0) s_bound[wave] = bound;
+    // each wavefront's share of n_select, the smallest of which n_select threads reach too: of many, the closer bound
+    unsigned share = 0;
+    if (A.n_select > kPickWaves / 2) share = nth_largest(order_of(low), (A.n_select + kPickWaves - 1) / kPickWaves);
+    if (lane == 0) {
+        s_bound[wave] = bound;
+        s_share[wave] = ~share;
+    }
     __syncthreads();
-    const double reach = (double)from_order(max(wave_max(s_bound[lane % kPickWaves]), order_of(-INFINITY)));
+    const unsigned closer = max(wave_max(s_bound[lane % kPickWaves]), ~wave_max(s_share[lane % kPickWaves]));
+    const double reach = (double)from_order(max(closer, order_of(-INFINITY)));
     auto list = [&](const Choice& c) {
         if (c.place == none || !(c.score >= reach)) return;
         const int at = atomicAdd(&s_count, 1);
@@ -395,7 +430,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
     };
 #pragma unroll
     for (int x = 0; x < kHeld; ++x) list(kept[x]);
-    for (unsigned i = kHeld * kPickThreads + tid; i < total; i += kPickThreads) list(choice(i));
+    others(list);
     __syncthreads();
     const int count = s_count;
     if (count <= kList) {                                 // at least n_select: the bound says so, or everything is in it
@@ -440,8 +475,8 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs A) {
     }
 }
 
-// Vocabulary per workgroup of the first launch: 8192, or 2048 where that leaves compute units without work (4 rows of 32000:
-// 4.9 us, 5.8 with 8192; 192 rows of 100003: 17 us with 8192, 23 with 2048).
+// Vocabulary per workgroup of the first launch: 8192, or 2048 where that leaves compute units without work (both
+// launches and the histories, 4 rows of 32000: 10.5 us, 11.4 with 8192; 192 rows of 100003: 23 us with 8192, 28 with 2048).
 static int pieces_of(size_t rows, int vocab) { return rows * (((size_t)vocab + 8191) / 8192) >= 256 ? 4 : 1; }
 static size_t slices_of(size_t rows, int vocab) {
     const size_t slice = (size_t)pieces_of(rows, vocab) * kBeamThreads * 8;
@@ -522,12 +557,14 @@ int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, con
     A.end_token = end_token;
     A.n_slices = (int)slices;
     A.slice = pieces * kBeamThreads * 8;
-    while ((1 << A.groups_log2) < n_select) ++A.groups_log2;
     const dim3 grid((unsigned)slices, (unsigned)rows);
     if (pieces == 4) beam_rows_kernel<4><<<grid, kBeamThreads, 0, stream()>>>(A);
     else beam_rows_kernel<1><<<grid, kBeamThreads, 0, stream()>>>(A);
     TL_CHECK_LAUNCH("beam_rows_kernel");
-    beam_pick_kernel<<<n_batch, kPickThreads, n_beams * (sizeof(double) + sizeof(int)), stream()>>>(A);
+    // 512 threads where they hold all continuations and have a wavefront for each beam (4 beams x 32000: 9.8 us, 10.1 with 1024)
+    const size_t lds = n_beams * (sizeof(double) + sizeof(int));
+    if (n_beams <= 8 && per_row * n_beams <= kHeld * 512) beam_pick_kernel<512><<<n_batch, 512, lds, stream()>>>(A);
+    else beam_pick_kernel<1024><<<n_batch, 1024, lds, stream()>>>(A);
     TL_CHECK_LAUNCH("beam_pick_kernel");
     return TL_OK;
 }

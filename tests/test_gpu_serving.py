@@ -922,3 +922,21 @@ def test_the_current_device_and_stream_are_checked(dev):
         assert torch.equal(pool, want) and lens.tolist() == [7]
     finally:
         dev.bind_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("n", [1, 8, 9, 64])
+def test_beam_select_when_the_bound_is_loose(dev, n):
+    """A quarter of each slice low, so that its wavefront's share is no bound for the rest; masks that leave fewer tokens than are
+    selected; slices of every length at the end."""
+    beams = 3
+    scores = torch.tensor([-1.0, -1.5, -1.25], device="cuda")
+    for vocab in (8192 * 86, 20000):                               # both slice lengths
+        for part in range(4):
+            low = rand((beams, vocab), 6 + part).abs()
+            low.view(beams, -1, 8)[:, torch.arange(vocab // 8, device="cuda") % 256 // 64 == part] -= 20
+            check_select(dev, low, scores, None, beams, 2, n)
+    for vocab in (2049, 2048 + 511, 2048 + 1791, 2048 + 1792, 4095, 4096):
+        masked = torch.full((beams, vocab), -math.inf, dtype=torch.float16, device="cuda")
+        masked[:, torch.randperm(vocab, generator=torch.Generator().manual_seed(vocab))[:5].cuda()] = rand((beams, 5), 3)
+        check_select(dev, masked, scores, None, beams, 2, n)
+        check_select(dev, rand((beams, vocab), 4), scores, None, beams, 2, n)

@@ -416,8 +416,8 @@ int tl_rotary_frequencies(double* host_out, int rotary_dim, double base, int sca
  * the rest of the head is copied.  freq: rotary_dim/2 DEVICE doubles.  Angles in fp64, the rotation in fp32, one rounding
  * (tl_apply_rotary_emb_f16 reproduces the reference's rounding after every operation instead).  Rows of n_heads * head_dim
  * elements, in_stride / out_stride elements apart; any head_dim, even rotary_dim <= head_dim, any int32 position.
- * out == in with equal strides is allowed.  16-byte accesses where pointers and strides allow them and rotary_dim is a
- * multiple of 8 (interleaved) or 16 (half) with head_dim % 8 == 0, else element by element. */
+ * out == in with equal strides is allowed.  Accesses of 16, 8 or 4 bytes: the widest that divides the addresses, the row strides,
+ * the head and the rotated part (each half of it for the half layout); else element by element. */
 int tl_rotary_f16(void* out, size_t out_stride, const void* in, size_t in_stride, const int* positions, const double* freq, int rotary_dim,
                   int layout, float magnitude, int n_tokens, int n_heads, int head_dim);
 

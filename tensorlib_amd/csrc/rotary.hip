@@ -7,7 +7,7 @@
 // and the rotation itself are fp32, rounded to half once.
 //
 // Bound by memory: every value is read and written once (4 bytes), the positions, frequencies and tables come from L2.
-// 16001 prompt tokens of 32 query and 8 kv heads of 128 take 71 us, 5.5 TB/s; a single token 3.4 us, a launch.
+// 16001 prompt tokens of 32 query and 8 kv heads of 128 take 70 us, 5.6 TB/s; a single token 3.4 us, a launch.
 #include <cmath>
 
 #include "paged.h"
@@ -70,48 +70,51 @@ __device__ __forceinline__ long slot_of(const RotaryArgs& A, size_t token, int p
     return (long)((size_t)page * A.cache.page_stride + (size_t)row * A.cache.row_stride);
 }
 
-// One thread: one unit of `ROWS` head rows of a token.  A unit is two 16-byte pieces whose elements pair up (HALF,
-// rotary_dim % 16 == 0), or one piece of four adjacent pairs (rotary_dim % 8 == 0); behind the rotated part, one piece
-// that is copied.  The rows of a thread share their angles, and their loads are in flight together.  STREAM: loads and
-// stores that do not settle in the caches.
-template <bool HALF, int ROWS, bool STREAM>
+// One thread: one unit of `ROWS` head rows of a token.  A unit is two pieces of VEC elements that pair up (HALF, rotary_dim a
+// multiple of 2 VEC), or one of VEC / 2 adjacent pairs (rotary_dim a multiple of VEC); behind the rotated part, one piece
+// that is copied.  The rows of a thread share their angles, and their loads are in flight together.
+template <bool HALF, int VEC, int ROWS, bool STREAM_IN, bool STREAM_OUT>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs A) {
+    typedef _Float16 piece __attribute__((ext_vector_type(VEC)));
     const unsigned id = blockIdx.x * 256u + threadIdx.x;
     if (id >= A.total) return;
     unsigned unit, group;
     const unsigned token = A.by_groups.divmod(A.by_units.divmod(id, unit), group);
     const int position = A.positions[token];
-    const int pairs8 = HALF ? A.rotary_dim / 16 : A.rotary_dim / 8;     // units of the rotated part
-    const bool turned = (int)unit < pairs8;
-    const int at = turned ? (int)unit * 8 : (HALF ? (int)unit * 8 + A.rotary_dim / 2 : (int)unit * 8);
+    const int pairing = HALF ? A.rotary_dim / (2 * VEC) : A.rotary_dim / VEC;     // units of the rotated part
+    const bool turned = (int)unit < pairing;
+    const int at = turned || !HALF ? (int)unit * VEC : (int)unit * VEC + A.rotary_dim / 2;
     const int other = at + A.rotary_dim / 2;
     const int n_rows = A.n_heads + 2 * A.n_kv;
     const long slot = (int)(group * ROWS + ROWS) > A.n_heads ? slot_of(A, token, position) : -1;
 
     auto load = [](const half_t* p) {
-        const half8_t* v = reinterpret_cast<const half8_t*>(p);
-        return STREAM ? __builtin_nontemporal_load(v) : *v;
+        const piece* v = reinterpret_cast<const piece*>(p);
+        return STREAM_IN ? __builtin_nontemporal_load(v) : *v;
     };
-    auto store = [](half_t* p, half8_t x) {
-        half8_t* v = reinterpret_cast<half8_t*>(p);
-        if (STREAM) __builtin_nontemporal_store(x, v);
+    auto store = [](half_t* p, piece x) {
+        piece* v = reinterpret_cast<piece*>(p);
+        if (STREAM_OUT) __builtin_nontemporal_store(x, v);
         else *v = x;
     };
     Row r[ROWS];
-    half8_t a[ROWS], b[ROWS];
+    piece a[ROWS], b[ROWS];
+    bool any = false;
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
         const int row = (int)group * ROWS + j;
         r[j] = row < n_rows ? row_of(A, token, row, slot) : Row{nullptr, nullptr, false};
+        any |= r[j].rotated;
         if (r[j].dst) {
             a[j] = load(r[j].src + at);
             if (HALF && turned) b[j] = load(r[j].src + other);
         }
     }
-    float c[8], s[8];
-    if (turned) {
+    constexpr int ANGLES = HALF ? VEC : VEC / 2;
+    float c[ANGLES], s[ANGLES];
+    if (turned && any) {
 #pragma unroll
-        for (int i = 0; i < (HALF ? 8 : 4); ++i) turn(position, A.freq[HALF ? at + i : at / 2 + i], A.magnitude, c[i], s[i]);
+        for (int i = 0; i < ANGLES; ++i) turn(position, A.freq[HALF ? at + i : at / 2 + i], A.magnitude, c[i], s[i]);
     }
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
@@ -119,14 +122,14 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs A) {
         if (turned && r[j].rotated) {
             if constexpr (HALF) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < ANGLES; ++i) {
                     const float x = (float)a[j][i], y = (float)b[j][i];
                     a[j][i] = (half_t)(x * c[i] - y * s[i]);
                     b[j][i] = (half_t)(x * s[i] + y * c[i]);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < ANGLES; ++i) {
                     const float x = (float)a[j][2 * i], y = (float)a[j][2 * i + 1];
                     a[j][2 * i] = (half_t)(x * c[i] - y * s[i]);
                     a[j][2 * i + 1] = (half_t)(x * s[i] + y * c[i]);
@@ -167,19 +170,37 @@ __global__ void __launch_bounds__(256) rotary_pairs_kernel(RotaryArgs A, int int
     r.dst[i1] = (half_t)y;
 }
 
-// From this many values on, two rows per thread and accesses past the caches (128 dims, 32 + 8 + 8 heads: 512 tokens 5.5 us
-// either way, 1024: 7.3 against 9.2, 16001: 71 against 84 us, 5.5 TB/s); below, one row and plain accesses (64 tokens 3.6
-// against 4.2 us).
-constexpr double kStreamValues = 4194304.0;
+static uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-static int launch_rotary(RotaryArgs& A, int n_tokens, int layout, bool vectors, const char* what) {
+// From this many values on two rows per thread, and stores past the caches (1024 tokens of 32 + 8 + 8 heads of 128: 7.1 us, 9.2 the
+// other way; 16000 of 8 + 8 + 8 of 96: 31 against 41); below, one row and plain accesses (64 tokens 3.6 against 4.2 us).
+constexpr double kManyValues = 4194304.0;
+// From this many on what is read and written exceeds the last-level cache.  Loads go past it too if a request's pieces make
+// whole lines (16001 tokens of 32 + 8 + 8 heads of 128: 69 us, 72 with plain loads).  Where a head is two halves that pair up and
+// not whole half lines, plain stores are better (40000 of 8 + 8 + 8 of 96: 84 against 98 us), at an odd number of pieces always (16000 of
+// 8 + 8 + 8 of 80: 36 against 45).
+constexpr double kPastCache = 67108864.0;
+
+template <bool HALF, int VEC>
+static void launch_rotary_pieces(const RotaryArgs& A, unsigned blocks, bool many, bool in, bool out) {
+    if (!many) rotary_kernel<HALF, VEC, 1, false, false><<<blocks, 256, 0, stream()>>>(A);
+    else if (VEC == 8 && in) rotary_kernel<HALF, VEC, 2, VEC == 8, true><<<blocks, 256, 0, stream()>>>(A);
+    else if (HALF && VEC == 8 && !out) rotary_kernel<HALF, VEC, 2, false, !(HALF && VEC == 8)><<<blocks, 256, 0, stream()>>>(A);
+    else rotary_kernel<HALF, VEC, 2, false, true><<<blocks, 256, 0, stream()>>>(A);
+}
+
+// alignment: all addresses and row strides in bytes, or-ed: a power of two that divides it divides them all.
+static int launch_rotary(RotaryArgs& A, int n_tokens, int layout, uintptr_t alignment, const char* what) {
     const bool half = layout == TL_ROTARY_HALF;
     const long n_rows = A.n_heads + 2L * A.n_kv;
-    vectors = vectors && A.head_dim % 8 == 0 && A.rotary_dim % (half ? 16 : 8) == 0;
-    const int units = vectors ? (half ? A.head_dim / 8 - A.rotary_dim / 16 : A.head_dim / 8) : (int)((A.head_dim + 1L) / 2);
-    const bool stream_ = vectors && (double)n_tokens * n_rows * A.head_dim >= kStreamValues;
-    const int rows = stream_ ? 2 : 1;
-    const long groups = (n_rows + rows - 1) / rows;
+    int vec = 8;                          // the widest pieces that fit
+    while (vec > 1 && (alignment % (2u * vec) || A.head_dim % vec || A.rotary_dim % (half ? 2 * vec : vec))) vec /= 2;
+    const int units = vec == 1 ? (int)((A.head_dim + 1L) / 2) : half ? (A.head_dim - A.rotary_dim / 2) / vec : A.head_dim / vec;
+    const double values = (double)n_tokens * n_rows * A.head_dim;
+    const bool many = vec > 1 && values >= kManyValues, past = values >= kPastCache;
+    const int run = half ? A.rotary_dim / 2 : A.head_dim;      // elements next to each other in one request
+    const bool in = past && run % 64 == 0 && A.head_dim % 64 == 0, out = !half || A.rotary_dim < A.head_dim || run % (past ? 32 : 16) == 0;
+    const long groups = many ? (n_rows + 1) / 2 : n_rows;
     const double total = (double)n_tokens * groups * units;
     if (total >= 2147483648.0 || n_rows > 0x7fffffff)
         return set_error(TL_ELIMIT, "%s: %d tokens of %ld heads of %d are too many for one call", what, n_tokens, n_rows, A.head_dim);
@@ -188,16 +209,10 @@ static int launch_rotary(RotaryArgs& A, int n_tokens, int layout, bool vectors, 
     A.by_units = FastDiv((unsigned)units);
     A.by_groups = FastDiv((unsigned)groups);
     const unsigned blocks = (A.total + 255u) / 256u;
-    if (!vectors) {
-        rotary_pairs_kernel<<<blocks, 256, 0, stream()>>>(A, half ? 0 : 1);
-        TL_CHECK_LAUNCH("rotary_pairs_kernel");
-    } else {
-        if (half && stream_) rotary_kernel<true, 2, true><<<blocks, 256, 0, stream()>>>(A);
-        else if (half) rotary_kernel<true, 1, false><<<blocks, 256, 0, stream()>>>(A);
-        else if (stream_) rotary_kernel<false, 2, true><<<blocks, 256, 0, stream()>>>(A);
-        else rotary_kernel<false, 1, false><<<blocks, 256, 0, stream()>>>(A);
-        TL_CHECK_LAUNCH("rotary_kernel");
-    }
+    if (vec == 1) rotary_pairs_kernel<<<blocks, 256, 0, stream()>>>(A, half ? 0 : 1);
+    else if (half) (vec == 8 ? launch_rotary_pieces<true, 8> : vec == 4 ? launch_rotary_pieces<true, 4> : launch_rotary_pieces<true, 2>)(A, blocks, many, in, out);
+    else (vec == 8 ? launch_rotary_pieces<false, 8> : vec == 4 ? launch_rotary_pieces<false, 4> : launch_rotary_pieces<false, 2>)(A, blocks, many, in, out);
+    TL_CHECK_LAUNCH("rotary_kernel");
     return TL_OK;
 }
 
@@ -266,8 +281,8 @@ int tl_rotary_f16(void* out, size_t out_stride, const void* in, size_t in_stride
     A.head_dim = head_dim;
     A.rotary_dim = rotary_dim;
     A.magnitude = magnitude;
-    const bool vectors = aligned16(out) && aligned16(in) && (n_tokens == 1 || (in_stride % 8 == 0 && out_stride % 8 == 0));
-    return launch_rotary(A, n_tokens, layout, vectors, "tl_rotary_f16");
+    const uintptr_t strides = n_tokens == 1 ? 0 : 2 * (in_stride | out_stride);
+    return launch_rotary(A, n_tokens, layout, address(out) | address(in) | strides, "tl_rotary_f16");
 }
 
 int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v, size_t v_stride,
@@ -309,9 +324,8 @@ int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const vo
     A.head_dim = cache->head_dim;
     A.rotary_dim = rotary_dim;
     A.magnitude = magnitude;
-    const bool vectors = aligned16(q_out) && aligned16(q) && aligned16(k) && aligned16(v) &&
-                         (n_tokens == 1 || (q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0));
-    return launch_rotary(A, n_tokens, layout, vectors, what);
+    const uintptr_t strides = n_tokens == 1 ? 0 : 2 * (q_stride | k_stride | v_stride);
+    return launch_rotary(A, n_tokens, layout, address(q_out) | address(q) | address(k) | address(v) | strides, what);
 }
 
 }  // extern "C"

@@ -82,6 +82,46 @@ def test_rotary(dev, layout, n, h, d, rd):
     within(dev.rotary(odd, positions, freq, layout, 1.25), want, 8e-7 * size, "rotary, misaligned")
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("offset,row,h,d,rd", [(0, 0, 3, 80, 20), (2, 0, 2, 64, 64), (4, 4, 2, 64, 64), (4, 2, 3, 96, 24), (0, 4, 3, 40, 40), (6, 8, 2, 128, 64),
+                                               (8, 12, 2, 16, 16), (0, 2, 1, 12, 8), (2, 6, 5, 10, 4), (1, 8, 2, 32, 32), (8, 1, 2, 32, 32), (4, 0, 7, 20, 12)])
+def test_rotary_at_every_alignment(dev, layout, offset, row, h, d, rd):
+    """Elements that the first row and the rows after it are off a multiple of 16 bytes, in and out; what lies around the rows
+    stays."""
+    n, width = 67, (h * d + 7) // 8 * 8 + 8
+    x, out = (rand(n * (width + row) + 16, s) for s in (1, 2))
+    view = lambda t: torch.as_strided(t, (n, h, d), (width + row, d, 1), offset)  # noqa: E731
+    positions = ints(np.random.RandomState(d).randint(0, 100000, n))
+    freq = dev.rotary_frequencies(rd)
+    want, size = rotated(view(x), positions, freq, layout, 1.0)
+    kept = out.clone()
+    dev.rotary(view(x), positions, freq, layout, out=view(out))
+    within(view(out), want, 8e-7 * size, "rotary")
+    view(kept).copy_(view(out))
+    assert torch.equal(out, kept)
+
+
+@pytest.mark.parametrize("n,h,kv,d,rd,layout", [(3000, 8, 8, 96, 24, "half"), (3000, 8, 8, 80, 20, "half"), (3000, 9, 8, 80, 80, "half"), (3000, 8, 8, 96, 96, "half"), (3000, 8, 8, 80, 20, "interleaved"),
+                                               (2000, 32, 2, 64, 64, "interleaved"), (29000, 8, 8, 96, 96, "half"), (22000, 9, 8, 128, 128, "half"), (22000, 8, 8, 128, 64, "interleaved"),
+                                               (35000, 8, 8, 80, 40, "half")])
+def test_rotary_of_many_tokens(dev, n, h, kv, d, rd, layout):
+    """Large batches move their values otherwise, and compute the same."""
+    page, step = 16, 1000
+    q, k, v = rand((n, h, d), 1), rand((n, kv, d), 2), rand((n, kv, d), 3)
+    positions, n_pages = torch.arange(n, dtype=torch.int32, device="cuda"), -(-n // page)
+    tables = torch.randperm(n_pages, generator=torch.Generator().manual_seed(1)).int().cuda()[None]
+    seq_ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    freq = dev.rotary_frequencies(rd)
+    kp, vp = (torch.zeros((n_pages, page, kv, d), dtype=torch.float16, device="cuda") for _ in range(2))
+    got = dev.rotary_paged(q, k, v, positions, seq_ids, freq, kp, vp, tables, layout)
+    for a in range(0, n, step):                                        # small calls, checked above
+        part = slice(a, a + step)
+        assert torch.equal(got[part], dev.rotary(q[part], positions[part], freq, layout)), a
+        rows = positions[part].long()
+        pages = tables[0][rows // page].long()
+        assert torch.equal(kp[pages, rows % page], dev.rotary(k[part], positions[part], freq, layout)) and torch.equal(vp[pages, rows % page], v[part]), a
+
+
 def test_rotary_far_negative_and_special_values(dev):
     n, h, d = 6, 2, 64
     x = rand((n, h, d), 3)

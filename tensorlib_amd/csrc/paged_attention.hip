@@ -16,7 +16,7 @@
 // layouts that need no exchange at all; its rate made 0.9 us of a 32-position turn: 13.7 against 12.4 us for 1 x 2048
 // positions of 32 heads, 108 against 92 us for 16 x 8000 positions of 256 dims.)
 //
-// Measured (one pass, both launches): 64 sequences of 65 to 4097 positions, 32 heads on 8 of 128: 114 us = 4.85 TB/s; in
+// Measured (one pass, both launches): 64 sequences of 65 to 4097 positions, 32 heads on 8 of 128: 106 us = 5.2 TB/s; in
 // the middle of the launch the memory runs at 6.0, the rest is the first requests' and the last workgroups' time.
 // 4 sequences of 100001 to 131072, 64 heads on 8: 320 us = 5.95 TB/s.  1 x 2048, 32 heads: 12.0 us, of which the two
 // launches of an empty problem take 8.
@@ -46,7 +46,7 @@ struct PagedAttnArgs {
     float* part_o;                        // [seq][split][head][head_dim]
     float2* part_ml;                      // [seq][split][head] (max in log2 units, sum)
     FastDiv by_page, by_heads, by_splits; // grid: (kv head tile) fastest, then split, then sequence
-    int n_heads, group, group_tiles, max_len, chunk, n_splits;
+    int n_heads, group, group_tiles, max_len, chunk, n_splits, turn_heads;
     float scale_log2;
 };
 
@@ -85,7 +85,10 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
     __shared__ float s_ml[kWaves][2][kGroupTile];
 
     unsigned head_tile, split;
-    const unsigned seq = A.by_splits.divmod(A.by_heads.divmod(blockIdx.x, head_tile), split);
+    const unsigned pair = A.by_heads.divmod(blockIdx.x, head_tile), seq = A.by_splits.divmod(pair, split);
+    // Workgroups go to the eight dies in turn, so eight kv heads in order would leave each die with one of them, whose rows lie in
+    // one eighth of its L2's channels: the heads of each next pair start elsewhere.
+    if (A.turn_heads) A.by_heads.divmod(head_tile + (pair + pair / 2 + pair / 4) % 65536, head_tile);
     const int t0 = (int)split * A.chunk;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int col = lane % 16, grp = lane / 16;
@@ -391,8 +394,8 @@ __global__ void __launch_bounds__(THREADS) paged_attention_join_kernel(PagedAttn
 // unit goes through one after the other, 42 more for each workgroup it is given, 240 for the join (in units of 128 dims, fitted
 // to thirty sizes).  It cuts 1 x 4096 on 8 kv heads into chunks of 128 (10.2 us, 13.7 with 512), 1 x 131072 on one into 512
 // (20.5, 28.2 with 128), 2 x 60000 on 2 into 1024 (29.5, 37 with 128), and leaves 64 x 700 on 8 whole (29.5, 42 with 512).  With
-// more: 512, since the last workgroups of a ragged batch then end close together (64 of 65 to 4097 positions on 8: 114 us, 117
-// with 1024, 135 with 128), 1024 for long contexts, where the partials are what can be saved (4 x 131072: 320, 332 with 512),
+// more: 512, since the last workgroups of a ragged batch then end close together (64 of 65 to 4097 positions on 8, heads in order: 114 us,
+// 117 with 1024, 135 with 128), 1024 for long contexts, where the partials are what can be saved (4 x 131072: 320, 332 with 512),
 // and where it leaves sequences whole (200 x 600: 60, 87 with 512).
 static int chunk_of(int n_seqs, int head_tiles, int head_dim, int max_len) {
     constexpr double kUnits = 256.0;
@@ -480,6 +483,8 @@ int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_k
     A.n_heads = n_heads;
     A.max_len = max_len;
     A.scale_log2 = scale * kLog2e;
+    // 64 ragged sequences of 8 kv heads of 128: 106 us, 114 in order; with few workgroups 2 % the other way (3 x 9000: 27.3, 27.0)
+    A.turn_heads = blocks > 1024.0;
     // V past the caches if what the sequences may read is more than the 256 MB of the last-level one and one pass reads it
     // (4 x 131072: 320 against 352 us, 64 ragged sequences 115 against 121; a cache of 66 MB that had stayed there 24 against 21)
     const bool past = A.group_tiles == 1 && (double)n_seqs * max_len * cache->n_kv_heads * cache->head_dim * 4.0 >= 268435456.0;

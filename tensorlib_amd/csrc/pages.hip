@@ -385,6 +385,9 @@ struct CompactArgs {
     const int* refs;
     int *refs_out, *remap, *copy_src, *copy_dst, *count;
     int n_pages;
+    const int* tables;
+    int* tables_out;
+    size_t n_entries;
 };
 __device__ __forceinline__ void compact_apply(const CompactArgs& A, int movers, size_t i, size_t step) {
     const int first = movers ? A.copy_src[0] : A.n_pages, last = movers ? A.copy_dst[movers - 1] : -1;
@@ -403,14 +406,26 @@ __device__ __forceinline__ void compact_apply(const CompactArgs& A, int movers, 
         }
     }
 }
+// The tables' entries i, i + step, ..
+__device__ __forceinline__ void compact_tables(const CompactArgs& A, size_t i, size_t step) {
+    for (; i < A.n_entries; i += step) {
+        const int p = A.tables[i];
+        A.tables_out[i] = p >= 0 && p < A.n_pages ? A.remap[p] : p;
+    }
+}
+__global__ void __launch_bounds__(256) pages_remap_kernel(CompactArgs A) {
+    compact_tables(A, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
+}
 __global__ void __launch_bounds__(256) pages_compact_apply_kernel(CompactArgs A) {
     compact_apply(A, *A.count, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
 }
-// One workgroup: the live pages above the number of live pages move into the free ones below it, in page order.  WHOLE: and all
-// the rest for a pool that one workgroup is soon through with (1000 pages 5.6 against 6.9 us and a launch, 4096 7.9 against 8.2,
-// 8192 11.4 against 10.3).
+// One workgroup: the live pages above the number of live pages move into the free ones below it, in page order.  PARTS: and all
+// the rest for a pool that one workgroup is soon through with (2; 1000 pages 5.6 against 6.9 us and a launch, 4096 7.9 against
+// 8.2, 8192 11.4 against 10.3), the tables too (3; 1000 pages and 100 entries 4.5 against 5.7 us and a launch, 4096 entries 5.6
+// against 5.9, 16384 9.0 against 6.0).
 constexpr int kWholePages = 4096;
-template <bool WHOLE>
+constexpr size_t kWholeEntries = 4096;
+template <int PARTS>
 __global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(CompactArgs A) {
     const PageRange range(A.refs, A.n_pages);
     int before, mine = 0, holes_before, unused;
@@ -423,16 +438,13 @@ __global__ void __launch_bounds__(kThreads) pages_compact_plan_kernel(CompactArg
     range.visit(before, 0x7fffffff, mover, [&](int k, int p, int) { A.copy_src[k] = p; });
     range.visit(holes_before, 0x7fffffff, hole, [&](int k, int p, int) { A.copy_dst[k] = p; });
     if (threadIdx.x == 0) *A.count = movers;
-    if constexpr (WHOLE) {
+    if constexpr (PARTS >= 2) {
         __syncthreads();
         compact_apply(A, movers, threadIdx.x, kThreads);
     }
-}
-
-__global__ void __launch_bounds__(256) pages_remap_kernel(int* out, const int* in, const int* remap, int n_pages, size_t n) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const int p = in[i];
-        out[i] = p >= 0 && p < n_pages ? remap[p] : p;
+    if constexpr (PARTS >= 3) {
+        __syncthreads();
+        compact_tables(A, threadIdx.x, kThreads);
     }
 }
 
@@ -557,19 +569,18 @@ int tl_pages_compact(const int* tables, const int* refs, int* tables_out, int* r
     TL_REQUIRE(refs && refs_out && remap && copy_src && copy_dst && count && (n_seqs == 0 || (tables && tables_out)), "%s: null pointer", what);
     TL_REQUIRE(refs_out != refs, "%s: the new reference counts must not lie over the old ones", what);
     TL_ENSURE_INIT();
-    const CompactArgs A{refs, refs_out, remap, copy_src, copy_dst, count, n_pages};
-    if (n_pages <= kWholePages) {
-        pages_compact_plan_kernel<true><<<1, kThreads, 0, stream()>>>(A);
-        TL_CHECK_LAUNCH("pages_compact_plan_kernel");
-    } else {
-        pages_compact_plan_kernel<false><<<1, kThreads, 0, stream()>>>(A);
-        TL_CHECK_LAUNCH("pages_compact_plan_kernel");
+    const size_t n = (size_t)n_seqs * table_stride;
+    const CompactArgs A{refs, refs_out, remap, copy_src, copy_dst, count, n_pages, tables, tables_out, n};
+    const int parts = n_pages > kWholePages ? 1 : n > kWholeEntries ? 2 : 3;
+    auto plan = parts == 1 ? pages_compact_plan_kernel<1> : parts == 2 ? pages_compact_plan_kernel<2> : pages_compact_plan_kernel<3>;
+    plan<<<1, kThreads, 0, stream()>>>(A);
+    TL_CHECK_LAUNCH("pages_compact_plan_kernel");
+    if (parts < 2) {
         pages_compact_apply_kernel<<<ints_grid(n_pages), 256, 0, stream()>>>(A);
         TL_CHECK_LAUNCH("pages_compact_apply_kernel");
     }
-    const size_t n = (size_t)n_seqs * table_stride;
-    if (n > 0) {
-        pages_remap_kernel<<<ints_grid(n), 256, 0, stream()>>>(tables_out, tables, remap, n_pages, n);
+    if (parts < 3 && n > 0) {
+        pages_remap_kernel<<<ints_grid(n), 256, 0, stream()>>>(A);
         TL_CHECK_LAUNCH("pages_remap_kernel");
     }
     return TL_OK;

@@ -434,10 +434,10 @@ __global__ void __launch_bounds__(THREADS) beam_pick_kernel(BeamArgs A) {
     __syncthreads();
     const int count = s_count;
     if (count <= kList) {                                 // at least n_select: the bound says so, or everything is in it
-        // P threads count for each choice of the list (a quarter of the threads at least find work)
+        // Several threads count for each choice of a short list.  A list may be longer than the workgroup (512 threads, up to kList
+        // choices): then a thread takes two.  With parts > 1 there is one turn, and all of a choice's lanes are in it together.
         const int parts = count <= kPickThreads / 8 ? 8 : count <= kPickThreads / 4 ? 4 : 1;
-        const int i = tid / parts;
-        if (i < count) {
+        for (int i = tid / parts; i < count; i += kPickThreads) {
             const Choice c = s_list[i];
             int rank = 0;
             for (int k = tid % parts; k < count; k += parts) rank += better(s_list[k], c);

@@ -980,3 +980,56 @@ def test_beam_select_when_the_bound_is_loose(dev, n):
         masked[:, torch.randperm(vocab, generator=torch.Generator().manual_seed(vocab))[:5].cuda()] = rand((beams, 5), 3)
         check_select(dev, masked, scores, None, beams, 2, n)
         check_select(dev, rand((beams, vocab), 4), scores, None, beams, 2, n)
+
+
+# ------------------------------------------------------------------------------------------------ long lists of the pick
+
+def select_into(dev, logits, scores, finished, n_beams, end, n):
+    """tl_beam_select_f16 itself, with outputs that hold something beforehand: a place that is not written shows."""
+    import ctypes
+    rows, vocab = logits.shape
+    batch = rows // n_beams
+    out = (torch.full((batch * n,), 12345.0, device="cuda"), ints([-77] * (batch * n)), ints([-99] * (batch * n)))
+    ws = torch.empty(dev.beam_select_workspace(batch, n_beams, vocab, n), dtype=torch.uint8, device="cuda")
+    p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    rc = dev.lib.tl_beam_select_f16(p(out[0]), p(out[1]), p(out[2]), p(logits), logits.stride(0), p(scores), p(finished), batch, n_beams, vocab, n, end, p(ws), ws.numel())
+    assert rc == 0, dev.lib.tl_last_error()
+    return out
+
+
+def check_select_into(dev, logits, scores, finished, n_beams, end, n):
+    """Tolerance of a score: half an fp32 step, and the logarithm of a row's sum, whose exponentials are good to an ulp (2^-23) and
+    whose additions within a thread are fp32, eight roundings in turn (8 * 2^-24): below 2^-20 together."""
+    want = select(logits, scores, finished, n_beams, end, n)
+    got = select_into(dev, logits, scores, finished, n_beams, end, n)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    fin = torch.isfinite(want[0])
+    assert torch.equal(got[0][~fin].double(), want[0][~fin])
+    off = (got[0].double() - want[0]).abs()[fin]
+    assert bool((off <= 2.0 ** -24 * want[0][fin].abs() + 2.0 ** -20).all()), float(off.max())
+
+
+@pytest.mark.parametrize("batch,beams,vocab,n,allowed", [(1, 4, 128256, 4, (100, 60000)), (1, 4, 50257, 8, (7, 50256)), (1, 8, 32000, 8, (31999,)), (1, 4, 100003, 4, (0, 99999)),
+                                                         (24, 8, 100003, 8, (70001,)), (3, 5, 32000, 10, (2, 16000, 31000))])
+def test_beam_select_under_a_mask_that_leaves_a_few_tokens(dev, batch, beams, vocab, n, allowed):
+    """Constrained decoding: all but a few tokens at -inf, the same ones in every beam. Most candidates are at -inf, too many
+    threads have nothing better for a bound, and hundreds of candidates are ranked; the best beam is the last one."""
+    rows = batch * beams
+    logits = torch.full((rows, vocab), -math.inf, dtype=torch.float16, device="cuda")
+    logits[:, list(allowed)] = rand((rows, len(allowed)), 5)
+    finished = (torch.arange(rows) % 3 == 1).cuda()
+    for scores in (torch.arange(rows, device="cuda") / 4.0 - 60.0, -torch.arange(rows, device="cuda") / 4.0):
+        check_select_into(dev, logits, scores, None, beams, 2, n)
+        check_select_into(dev, logits, scores, finished, beams, 2, n)
+
+
+@pytest.mark.parametrize("beams,slices,n,rest", [(8, 8, 8, 2048), (3, 9, 19, 19), (8, 16, 8, 8), (3, 11, 31, 2047), (5, 5, 41, 100), (7, 11, 13, 300), (1, 16, 64, 64), (8, 10, 8, 9), (1, 8, 64, 64),
+                                                  (1, 17, 61, 61)])
+@pytest.mark.parametrize("step", [0.0, 2.0 ** -20, -2.0 ** -20])
+def test_beam_select_of_lists_of_any_length(dev, beams, slices, n, rest, step):
+    """Rows of equal logits: every candidate reaches the bound, so the list is as long as there are candidates (beams x slices x
+    n: 512, 513, 1024, 1023, 1025, 1001, 1024, 640, 512, 1037), whether the beams are equal, the last one the best or the first."""
+    vocab = (slices - 1) * 2048 + rest
+    logits = torch.full((beams, vocab), 1.5, dtype=torch.float16, device="cuda")
+    scores = -1.0 + step * torch.arange(beams, device="cuda", dtype=torch.float32)
+    check_select_into(dev, logits, scores, None, beams, 2, n)

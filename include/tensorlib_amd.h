@@ -433,11 +433,14 @@ int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const vo
 /* Attention of one token per sequence: out[b,h,:] = softmax(scale * q[b,h,:] . K[0:lens[b], g(h), :]^T) . V[0:lens[b], g(h), :]
  * with g(h) = h / (n_heads / n_kv_heads).  q rows of n_heads * head_dim elements are q_stride apart, out is dense.
  * lens counts the cached positions, the token's own among them; max_len is the caller's bound on it, which sizes the
- * launch and the workspace (tl_paged_attention_workspace bytes for the same sizes, 0 if it needs none; a smaller max_len may
- * need more; nothing in it has to be cleared or survives the call).  lens[b] <= 0 gives zeros; lens[b] beyond max_len or the table, or a page out of range among the
+ * launch and the workspace; nothing in that has to be cleared or survives the call.  tl_paged_attention_workspace bytes are enough
+ * for every call with these heads, at most n_seqs sequences and a bound of at most max_len; what one call of just these sizes
+ * needs is tl_paged_attention_workspace_of_call bytes (0 if none), which may be more for a smaller call.  lens[b] <= 0 gives
+ * zeros; lens[b] beyond max_len or the table, or a page out of range among the
  * pages it covers, gives NaN for that sequence.  Scores, weights and sums are fp32, one rounding at the end.
  * At most 65535 sequences.  out may be q if q is dense. */
 size_t tl_paged_attention_workspace(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len);
+size_t tl_paged_attention_workspace_of_call(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len);
 int tl_paged_attention_f16(void* out, const void* q, size_t q_stride, const tl_kv_pages* cache, const int* tables, size_t table_stride,
                            const int* lens, int n_seqs, int n_heads, int max_len, float scale, void* workspace, size_t workspace_bytes);
 

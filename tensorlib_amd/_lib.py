@@ -133,6 +133,7 @@ _PROTOS = {
     "tl_rotary_f16": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _i, _i, _f, _i, _i, _i]),
     "tl_rotary_kv_pages_f16": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _i, _i, _f, _i, _i, _kvp, _vp, _sz, _i]),
     "tl_paged_attention_workspace": (_sz, [_i, _i, _i, _i, _i]),
+    "tl_paged_attention_workspace_of_call": (_sz, [_i, _i, _i, _i, _i]),
     "tl_paged_attention_f16": (_i, [_vp, _vp, _sz, _kvp, _vp, _sz, _vp, _i, _i, _i, _f, _vp, _sz]),
     "tl_pages_fork": (_i, [_vp] * 10 + [_i, _i, _i, _i]),
     "tl_pages_extend": (_i, [_vp] * 5 + [_i, _i, _i, _i]),

@@ -20,6 +20,7 @@
 // the middle of the launch the memory runs at 6.0, the rest is the first requests' and the last workgroups' time.
 // 4 sequences of 100001 to 131072, 64 heads on 8: 320 us = 5.95 TB/s.  1 x 2048, 32 heads: 12.0 us, of which the two
 // launches of an empty problem take 8.
+#include <algorithm>
 #include <cmath>
 
 #include "paged.h"
@@ -390,6 +391,10 @@ __global__ void __launch_bounds__(THREADS) paged_attention_join_kernel(PagedAttn
     *reinterpret_cast<half4_t*>(A.out + ((size_t)seq * A.n_heads + h) * D + d) = r;
 }
 
+constexpr double kUnits = 256.0, kMany = 6 * kUnits;
+constexpr int kLongContext = 32768;
+static double dims_of(int head_dim) { return head_dim <= 64 ? 0.5 : head_dim <= 128 ? 1.0 : 2.0; }
+
 // Positions per workgroup.  With fewer workgroups than six times the 256 compute units, the least of: positions that the fullest
 // unit goes through one after the other, 42 more for each workgroup it is given, 240 for the join (in units of 128 dims, fitted
 // to thirty sizes).  It cuts 1 x 4096 on 8 kv heads into chunks of 128 (10.2 us, 13.7 with 512), 1 x 131072 on one into 512
@@ -398,11 +403,10 @@ __global__ void __launch_bounds__(THREADS) paged_attention_join_kernel(PagedAttn
 // 117 with 1024, 135 with 128), 1024 for long contexts, where the partials are what can be saved (4 x 131072: 320, 332 with 512),
 // and where it leaves sequences whole (200 x 600: 60, 87 with 512).
 static int chunk_of(int n_seqs, int head_tiles, int head_dim, int max_len) {
-    constexpr double kUnits = 256.0;
-    const double tiles = (double)n_seqs * head_tiles, dims = head_dim <= 64 ? 0.5 : head_dim <= 128 ? 1.0 : 2.0;
+    const double tiles = (double)n_seqs * head_tiles, dims = dims_of(head_dim);
     int best = kMaxChunk;
-    if (tiles * ceil(max_len / 512.0) * dims >= 6 * kUnits) {
-        if (max_len > kMaxChunk && max_len <= 32768) best = kMaxChunk / 2;
+    if (tiles * ceil(max_len / 512.0) * dims >= kMany) {
+        if (max_len > kMaxChunk && max_len <= kLongContext) best = kMaxChunk / 2;
     } else {
         double least = 1e300;
         for (int chunk = kMaxChunk; chunk >= kMinChunk; chunk /= 2) {
@@ -416,6 +420,19 @@ static int chunk_of(int n_seqs, int head_tiles, int head_dim, int max_len) {
     }
     while (best > kMinChunk && best / 2 >= max_len) best /= 2;
     return best;
+}
+// At least the chunks, of all sequences together, of any call with at most n_seqs sequences and a bound of at most max_len.  Calls with
+// many workgroups have chunks of 512 up to kLongContext and of 1024 beyond.  The others have n_seqs * head_tiles * ceil(max_len / 512) below
+// kMany / dims, and in chunks of 128, the smallest, at most four times as many.  Up to 128 positions are one chunk.
+static size_t most_chunks(int n_seqs, int head_tiles, int head_dim, int max_len) {
+    if (max_len <= kMinChunk) return 0;
+    const double n = n_seqs, most = kMany / (dims_of(head_dim) * head_tiles);
+    double chunks = n * ceil(max_len / (double)kMinChunk);
+    if (n * ceil(max_len / 512.0) >= most) {
+        const double many = n * std::max(ceil(std::min(max_len, kLongContext) / 512.0), ceil(max_len / (double)kMaxChunk));
+        chunks = std::min(chunks, std::max(many, ceil(4.0 * most)));
+    }
+    return (size_t)(ceil(chunks / n) * n);
 }
 static int group_tiles_of(int n_heads, int n_kv_heads) { return (n_heads / n_kv_heads + kGroupTile - 1) / kGroupTile; }
 
@@ -432,6 +449,11 @@ static void launch_paged_attention(const PagedAttnArgs& A, unsigned blocks, bool
 extern "C" {
 
 size_t tl_paged_attention_workspace(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len) {
+    if (n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || head_dim <= 0 || max_len <= 0) return 0;
+    return tl::most_chunks(n_seqs, n_kv_heads * tl::group_tiles_of(n_heads, n_kv_heads), head_dim, max_len) * n_heads * ((size_t)head_dim + 2) * sizeof(float);
+}
+
+size_t tl_paged_attention_workspace_of_call(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len) {
     if (n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || head_dim <= 0 || max_len <= 0) return 0;
     const int chunk = tl::chunk_of(n_seqs, n_kv_heads * tl::group_tiles_of(n_heads, n_kv_heads), head_dim, max_len);
     const size_t splits = ((size_t)max_len + chunk - 1) / chunk;

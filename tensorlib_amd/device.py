@@ -530,7 +530,8 @@ class HipDevice:
         return self._front.paged_attention(self.ordinal, q, k_pages, v_pages, tables, lens, scale, max_len, out, workspace)
 
     def paged_attention_workspace(self, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int) -> int:
-        """Bytes of workspace paged_attention needs for these sizes; 0 where it needs none."""
+        """Bytes of workspace that are enough for paged_attention with these heads, up to n_seqs sequences and any max_len up to this
+        one; 0 where it needs none."""
         return self.lib.tl_paged_attention_workspace(n_seqs, n_heads, n_kv_heads, head_dim, max_len)
 
     def pages_fork(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int):

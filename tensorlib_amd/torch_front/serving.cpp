@@ -254,7 +254,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.may_allocate();
     const at::Tensor out = a.none(8) ? at::empty({b, h, cache.head_dim}, q.options()) : a.head_rows(8, "out", b, h, cache.head_dim);
     if (!out.is_contiguous()) fail(PyExc_ValueError, "out must be contiguous");
-    const Workspace ws(a, 9, a.none(9) ? tl_paged_attention_workspace(seqs, h, cache.n_kv_heads, cache.head_dim, max_len) : 0, q);
+    const Workspace ws(a, 9, a.none(9) ? tl_paged_attention_workspace_of_call(seqs, h, cache.n_kv_heads, cache.head_dim, max_len) : 0, q);
     call("tl_paged_attention_f16", tl_paged_attention_f16, out.data_ptr(), q.data_ptr(), (size_t)q.stride(0), &cache, ptr<int>(tables), (size_t)width,
          ptr<int>(lens), seqs, h, max_len, scale, ws.p, ws.bytes);
     return THPVariable_Wrap(out);

@@ -1033,3 +1033,17 @@ def test_beam_select_of_lists_of_any_length(dev, beams, slices, n, rest, step):
     logits = torch.full((beams, vocab), 1.5, dtype=torch.float16, device="cuda")
     scores = -1.0 + step * torch.arange(beams, device="cuda", dtype=torch.float32)
     check_select_into(dev, logits, scores, None, beams, 2, n)
+
+
+def test_one_workspace_for_every_bound_and_batch(dev):
+    """A workspace sized once for the limit of a program serves its shorter bounds and smaller batches."""
+    h, kv, d, page, lens = 32, 8, 128, 16, [20000, 700, 4097]
+    tables, n_pages = tables_for(lens, page)
+    kp, vp = paged_cache(n_pages, page, kv, d, "row")
+    q = rand((3, h, d), 8)
+    ws = torch.empty(dev.paged_attention_workspace(3, h, kv, d, 131072), dtype=torch.uint8, device="cuda")
+    for rows in (slice(0, 3), slice(0, 1), slice(1, 3), slice(1, 2)):
+        for bound in (20000, 25000, 73728, 131072):
+            args = q[rows], kp, vp, ints(tables[rows]), ints(lens[rows])
+            ws.fill_(255)                                          # NaN, whatever is read of it
+            assert torch.equal(dev.paged_attention(*args, max_len=bound, workspace=ws), dev.paged_attention(*args, max_len=bound)), (rows, bound)

@@ -3,6 +3,7 @@ frequencies: host code, no GPU. The C entry points check every argument before t
 made-up pointers come back with TL_EINVAL / TL_ELIMIT and a message."""
 import ctypes
 import math
+import re
 
 import numpy as np
 import pytest
@@ -201,3 +202,45 @@ def test_native_front_end_takes_device_tensors_only(name, arguments):
         entry()
     with pytest.raises(TypeError, match="ordinal"):
         entry("0", *[None] * (arguments - 1))
+
+
+# ------------------------------------------------------------------------------------------------ workspaces
+
+def needed(name, args):
+    """What a call asks for when its workspace is too small."""
+    rc, msg = call(name, *args)
+    assert rc == TL_EINVAL, (rc, msg)
+    return int(re.search(r"workspace of (\d+) bytes", msg).group(1))
+
+
+def attention_needs(n_seqs, n_heads, kv, dim, max_len):
+    c = cache(page_stride=16 * kv * dim, row_stride=kv * dim, head_stride=dim, n_kv_heads=kv, head_dim=dim)
+    args = changed(ATTENTION, cache=c, n_seqs=n_seqs, n_heads=n_heads, q_stride=n_heads * dim, max_len=max_len, ws=P, ws_bytes=0)
+    exact = _lib.lib().tl_paged_attention_workspace_of_call(n_seqs, n_heads, kv, dim, max_len)
+    if exact:           # then a call with none is refused; one that needs none would go on
+        assert needed("tl_paged_attention_f16", args) == exact
+    return exact
+
+
+@pytest.mark.parametrize("n_heads,kv,dim", [(32, 8, 128), (32, 32, 128), (8, 1, 64), (40, 1, 96), (64, 8, 256), (4, 4, 8), (66, 2, 136)])
+def test_an_attention_workspace_serves_every_smaller_call(n_heads, kv, dim):
+    """Fewer sequences and shorter bounds take smaller chunks, so one call alone can need more than a larger one."""
+    lib = _lib.lib()
+    rng = np.random.RandomState(n_heads + dim)
+    grew = False
+    for max_seqs, limit in ((1, 131072), (1, 40000), (3, 9000), (17, 131072), (64, 4097), (200, 700), (1000, 33000), (5, 130), (9, 128)):
+        enough = lib.tl_paged_attention_workspace(max_seqs, n_heads, kv, dim, limit)
+        assert enough % (n_heads * (dim + 2) * 4) == 0
+        lens = np.unique(np.concatenate([np.exp(rng.uniform(0, math.log(limit), 300)).astype(int), np.arange(1, limit // 128 + 1, max(1, limit // 128 // 300)) * 128, [limit]]))
+        for n in {1, min(2, max_seqs), max_seqs // 2, max_seqs - 1, max_seqs} - {0}:
+            largest = max(attention_needs(n, n_heads, kv, dim, int(x)) for x in lens if x <= limit)
+            assert largest <= enough, (n, max_seqs, limit)
+            grew |= largest > lib.tl_paged_attention_workspace_of_call(max_seqs, n_heads, kv, dim, limit)
+    assert grew          # a call with a smaller bound did need more
+    assert lib.tl_paged_attention_workspace(9, n_heads, kv, dim, 128) == 0
+
+
+@pytest.mark.parametrize("args", [(0, 4, 2, 64, 100), (4, 0, 2, 64, 100), (4, 4, 0, 64, 100), (4, 4, 3, 64, 100), (4, 4, 2, 0, 100), (4, 4, 2, 64, 0), (-1, 4, 2, 64, 100)])
+def test_workspaces_of_impossible_sizes(args):
+    assert _lib.lib().tl_paged_attention_workspace(*args) == 0
+    assert _lib.lib().tl_paged_attention_workspace_of_call(*args) == 0

@@ -478,7 +478,8 @@ int tl_pages_copy(void* pool, size_t plane_stride, size_t page_stride, size_t pa
  * token.  finished (bytes, may be NULL): a finished row continues only with end_token, at its own score.  Everything
  * else is at -inf and follows in the same order: other tokens of a finished row, all tokens of a row whose logits
  * hold NaN or +inf or nothing but -inf, or whose score is not finite.  Row sums and comparisons in fp64.
- * n_select <= 64, n_beams <= 1024, at most 65535 rows. */
+ * n_select <= 64, n_beams <= 1024, at most 65535 rows.  tl_beam_select_workspace bytes are enough for every call with at most as many
+ * requests, beams, tokens and continuations. */
 size_t tl_beam_select_workspace(int n_batch, int n_beams, int vocab, int n_select);
 int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, const void* logits, size_t logits_stride, const float* scores,
                        const uint8_t* finished, int n_batch, int n_beams, int vocab, int n_select, int end_token, void* workspace,

@@ -19,6 +19,7 @@
 // 24 requests of 8 beams over 100003 tokens: 13 + 6 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
 // for 7 us of the first launch, and its workgroups do not all run at a time).  1 request of 4 beams over 32000: 4 + 4 us,
 // two launches and their memory latencies.  64 beams over 100003, 64 selected: 120 us, most of it the second launch.
+#include <algorithm>
 #include <cmath>
 
 #include "paged.h"
@@ -477,11 +478,13 @@ __global__ void __launch_bounds__(THREADS) beam_pick_kernel(BeamArgs A) {
 
 // Vocabulary per workgroup of the first launch: 8192, or 2048 where that leaves compute units without work (both
 // launches and the histories, 4 rows of 32000: 10.5 us, 11.4 with 8192; 192 rows of 100003: 23 us with 8192, 28 with 2048).
-static int pieces_of(size_t rows, int vocab) { return rows * (((size_t)vocab + 8191) / 8192) >= 256 ? 4 : 1; }
-static size_t slices_of(size_t rows, int vocab) {
-    const size_t slice = (size_t)pieces_of(rows, vocab) * kBeamThreads * 8;
+constexpr size_t kManySlices = 256;
+static size_t slices_of(int pieces, int vocab) {
+    const size_t slice = (size_t)pieces * kBeamThreads * 8;
     return ((size_t)vocab + slice - 1) / slice;
 }
+static int pieces_of(size_t rows, int vocab) { return rows * slices_of(4, vocab) >= kManySlices ? 4 : 1; }
+static size_t slice_bytes(int n_select) { return sizeof(SliceStats) + (size_t)n_select * sizeof(unsigned); }
 
 struct AdvanceArgs {
     const int *history, *lens;
@@ -514,7 +517,9 @@ extern "C" {
 size_t tl_beam_select_workspace(int n_batch, int n_beams, int vocab, int n_select) {
     if (n_batch <= 0 || n_beams <= 0 || vocab <= 0 || n_select <= 0) return 0;
     const size_t rows = (size_t)n_batch * n_beams;
-    return rows * tl::slices_of(rows, vocab) * (sizeof(tl::SliceStats) + (size_t)n_select * sizeof(unsigned));
+    // Calls in short slices have fewer than kManySlices long ones, so at most four times as many.
+    const size_t few = std::min(rows * tl::slices_of(1, vocab), 4 * (tl::kManySlices - 1));
+    return std::max(rows * tl::slices_of(4, vocab), few) * tl::slice_bytes(n_select);
 }
 
 int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, const void* logits, size_t logits_stride, const float* scores,
@@ -533,10 +538,10 @@ int tl_beam_select_f16(float* scores_out, int* tokens_out, int* parents_out, con
     const size_t rows = (size_t)n_batch * n_beams;
     if (rows > 65535) return set_error(TL_ELIMIT, "%s: %zu rows, at most 65535", what, rows);
     const int pieces = pieces_of(rows, vocab);
-    const size_t slices = slices_of(rows, vocab);
+    const size_t slices = slices_of(pieces, vocab);
     const size_t per_row = slices * n_select > (size_t)n_select + 1 ? slices * n_select : (size_t)n_select + 1;
     if (per_row * n_beams >= (1u << 31)) return set_error(TL_ELIMIT, "%s: a vocabulary of %d is too large for %d beams", what, vocab, n_beams);
-    const size_t need = tl_beam_select_workspace(n_batch, n_beams, vocab, n_select);
+    const size_t need = rows * slices * slice_bytes(n_select);
     TL_REQUIRE(workspace && workspace_bytes >= need && aligned16(workspace), "%s: needs an aligned workspace of %zu bytes, got %zu", what, need,
                workspace ? workspace_bytes : (size_t)0);
     TL_ENSURE_INIT();

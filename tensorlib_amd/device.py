@@ -565,7 +565,7 @@ class HipDevice:
         return self._front.beam_select(self.ordinal, logits, scores, n_beams, finished, end_token, n_select, workspace)
 
     def beam_select_workspace(self, n_batch: int, n_beams: int, vocab: int, n_select: int) -> int:
-        """Bytes of workspace beam_select needs for these sizes."""
+        """Bytes of workspace that are enough for beam_select with these sizes and any smaller ones."""
         return self.lib.tl_beam_select_workspace(n_batch, n_beams, vocab, n_select)
 
     def beam_advance(self, history: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor | None, parents: torch.Tensor,

@@ -1047,3 +1047,14 @@ def test_one_workspace_for_every_bound_and_batch(dev):
             args = q[rows], kp, vp, ints(tables[rows]), ints(lens[rows])
             ws.fill_(255)                                          # NaN, whatever is read of it
             assert torch.equal(dev.paged_attention(*args, max_len=bound, workspace=ws), dev.paged_attention(*args, max_len=bound)), (rows, bound)
+
+
+def test_one_workspace_for_every_beam_batch(dev):
+    """A workspace sized once for the largest batch serves the smaller ones, whose rows are cut more finely."""
+    beams, vocab, most = 4, 100003, 12
+    logits, scores = rand((most * beams, vocab), 3, 2.5), -20 * torch.rand(most * beams, generator=torch.Generator().manual_seed(1)).cuda()
+    ws = torch.empty(dev.beam_select_workspace(most, beams, vocab, beams), dtype=torch.uint8, device="cuda")
+    for batch in (most, 5, 4, 2, 1):
+        ws.fill_(255)
+        args = logits[: batch * beams], scores[: batch * beams], beams
+        assert all(torch.equal(a, b) for a, b in zip(dev.beam_select(*args, workspace=ws), dev.beam_select(*args)))

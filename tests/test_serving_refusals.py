@@ -244,3 +244,18 @@ def test_an_attention_workspace_serves_every_smaller_call(n_heads, kv, dim):
 def test_workspaces_of_impossible_sizes(args):
     assert _lib.lib().tl_paged_attention_workspace(*args) == 0
     assert _lib.lib().tl_paged_attention_workspace_of_call(*args) == 0
+
+
+@pytest.mark.parametrize("beams", [1, 4, 8, 64])
+@pytest.mark.parametrize("vocab", [100, 8192, 8193, 32000, 100003, 300000])
+def test_a_beam_workspace_serves_every_smaller_call(beams, vocab):
+    """Few rows take shorter slices, so a call can need more than one with more rows."""
+    lib = _lib.lib()
+    for most in (1, 2, 5, 24, 100, 700):
+        for n in (1, beams, min(64, beams * vocab)):
+            enough = lib.tl_beam_select_workspace(most, beams, vocab, n)
+            batches = sorted({1, 2, most} | set(range(1, most, max(1, most // 60)))) if most > 1 else [1]
+            for smaller in (vocab, vocab // 2 + 1, max(n, vocab // 3)):
+                for b in batches:
+                    if b <= most and n <= beams * smaller:
+                        assert needed("tl_beam_select_f16", changed(SELECT, n_batch=b, n_beams=beams, vocab=smaller, logits_stride=smaller, n_select=n, ws_bytes=0)) <= enough, (b, most, n)

@@ -545,7 +545,7 @@ class HipDevice:
         return self._front.pages_extend(self.ordinal, tables, lens, refs, add, page_size)
 
     def pages_free(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor, page_size: int) -> None:
-        """Gives back the pages of the sequences with rows[i] true and empties them, in place."""
+        """Gives back the pages of the sequences with rows[i] true and empties them, in place; streams as in pages_copy."""
         self._front.pages_free(self.ordinal, tables, lens, refs, rows, page_size)
 
     def pages_compact(self, tables: torch.Tensor, refs: torch.Tensor):
@@ -555,7 +555,7 @@ class HipDevice:
 
     def pages_copy(self, pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, count: torch.Tensor | None = None) -> None:
         """pool [planes, pages, ..]: page src[i] of every plane to page dst[i], in place; ids of -1 are skipped, and pairs from
-        count[0] on."""
+        count[0] on. On a library stream that is not torch's current one it stays in line with that."""
         self._front.pages_copy(self.ordinal, pool, src, dst, count)
 
     def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, n_beams: int, finished: torch.Tensor | None = None, end_token: int = 2,

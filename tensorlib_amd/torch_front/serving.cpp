@@ -197,6 +197,49 @@ PyObject* pack(std::initializer_list<at::Tensor> tensors) {
     return result.release();
 }
 
+// Puts one call, which allocates nothing, in line with torch's current stream where the library enqueues on another one: behind
+// what was enqueued there so far, since that made the tensors, and ahead of what comes, since that reads them or has their
+// memory again once they are freed.  A capture on the library's stream has an order of its own; one on torch's alone would go
+// without the call.
+class InLine {
+    hipStream_t library_, torch_;
+    bool apart_;
+
+    static void check(hipError_t e) {
+        if (e == hipSuccess) return;
+        (void)hipGetLastError();           // reported here, not by the next call
+        fail(g_error, "ordering the library stream and torch's current stream failed: %s", hipGetErrorString(e));
+    }
+    static bool capturing(hipStream_t s) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (s) check(hipStreamIsCapturing(s, &status));       // the null stream never is
+        return status != hipStreamCaptureStatusNone;
+    }
+    static void follow(hipStream_t later, hipStream_t earlier) {
+        hipEvent_t event;
+        check(hipEventCreateWithFlags(&event, hipEventDisableTiming));
+        hipError_t e = hipEventRecord(event, earlier);
+        if (e == hipSuccess) e = hipStreamWaitEvent(later, event, 0);
+        (void)hipEventDestroy(event);      // what waits for it goes on doing so
+        check(e);
+    }
+
+public:
+    explicit InLine(const Args& a) {
+        a.on_device();
+        library_ = static_cast<hipStream_t>(tl_get_stream());
+        torch_ = c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.ordinal).stream();
+        apart_ = library_ != torch_ && !capturing(library_);
+        if (!apart_) return;
+        if (capturing(torch_))
+            fail(g_error, "torch's current stream is being captured and the library stream is another; call bind_stream(torch.cuda.current_stream()) first");
+        follow(library_, torch_);
+    }
+    void done() const {
+        if (apart_) follow(torch_, library_);
+    }
+};
+
 // (ordinal, x, positions, freq, layout, magnitude, out or None)
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -308,9 +351,10 @@ PyObject* pages_free(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Args a(args, n, 6, "pages_free");
     const PageState s(a, 1);
     const at::Tensor& rows = a.vector(4, "rows", at::kBool, s.rows);
-    a.on_device();
+    const InLine line(a);
     call("tl_pages_free", tl_pages_free, ptr<int>(s.tables), ptr<int>(s.lens), ptr<int>(s.refs), ptr<uint8_t>(rows), s.rows, s.width, s.pages,
          a.int32(5, "page_size"));
+    line.done();
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -346,9 +390,10 @@ PyObject* pages_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor& src = a.dense(2, "src", at::kInt, 1);
     const at::Tensor& dst = a.vector(3, "dst", at::kInt, src.size(0));
     const int* count = a.none(4) ? nullptr : ptr<int>(a.vector(4, "count", at::kInt, 1));
-    a.on_device();
+    const InLine line(a);
     call("tl_pages_copy", tl_pages_copy, pool.data_ptr(), (size_t)(pool.stride(0) * item), (size_t)(pool.stride(1) * item), (size_t)page_bytes,
          size32(pool.size(0), "pool"), size32(pool.size(1), "pool"), ptr<int>(src), ptr<int>(dst), count, size32(src.size(0), "src"));
+    line.done();
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }

@@ -1058,3 +1058,77 @@ def test_one_workspace_for_every_beam_batch(dev):
         ws.fill_(255)
         args = logits[: batch * beams], scores[: batch * beams], beams
         assert all(torch.equal(a, b) for a, b in zip(dev.beam_select(*args, workspace=ws), dev.beam_select(*args)))
+
+
+def test_calls_on_another_stream_than_torchs_stay_in_line(dev):
+    """pages_copy and pages_free may run on a library stream that is not torch's current one: behind what made their tensors
+    there, ahead of what reads them and of what has their memory next."""
+    pool, wait = rand((4, 60, 8, 64), 1), 20_000_000               # cycles, some ten milliseconds
+    src, dst = np.arange(0, 30), np.arange(59, 29, -1)
+    want = pool.clone()
+    want[:, dst] = pool[:, src]
+    tables, lens, refs, _ = state(40, 8, 12, 9, 10)
+    rows = np.arange(40) % 3 == 0
+    left = np.where(rows[:, None], -1, tables)
+    device_src, device_dst = ints(src), ints(dst)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    dev.bind_stream(side)
+    try:
+        for slow in (torch.cuda.current_stream(), side):
+            p, t, ln, r = torch.zeros_like(pool), ints(np.full_like(tables, -1)), ints(np.zeros_like(lens)), ints(np.zeros_like(refs))
+            values = [pool, ints(tables), ints(lens), ints(refs)]
+            torch.cuda.synchronize()
+            with torch.cuda.stream(slow):
+                torch.cuda._sleep(wait)
+            for to, x in zip((p, t, ln, r), values):
+                to.copy_(x)                                        # the operands are there only now
+            ids = device_src + 0, device_dst + 0
+            dev.pages_copy(p, *ids)
+            del ids
+            other = torch.full((30,), 7, dtype=torch.int32, device="cuda"), torch.full((30,), 7, dtype=torch.int32, device="cuda")
+            which = torch.as_tensor(rows, device="cuda")
+            dev.pages_free(t, ln, r, which, 8)
+            which.zero_()                                          # and its readers wait
+            got = [x.clone() for x in (p, t, ln, r)]
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want) and all(bool((o == 7).all()) for o in other)
+            assert np.array_equal(got[1].cpu().numpy(), left) and np.array_equal(got[2].cpu().numpy(), np.where(rows, 0, lens))
+            assert np.array_equal(got[3].cpu().numpy(), np.bincount(left[left >= 0], minlength=len(refs)))
+    finally:
+        dev.bind_stream(torch.cuda.current_stream())
+
+
+def test_captures_and_another_library_stream(dev):
+    """A capture of torch's stream would go without a call that the library enqueues elsewhere: refused, and the capture goes on.
+    A capture of the library's own stream records it, whatever torch's current stream is."""
+    pool, src, dst = rand((2, 6, 16), 1), ints([5, 1]), ints([3, 0])
+    kept, want = pool.clone(), pool.clone()
+    want[:, [3, 0]] = pool[:, [5, 1]]
+    state_ = ints([[0, 1]]), ints([7]), ints([1, 1, 0]), torch.ones(1, dtype=torch.bool, device="cuda")
+    side, main = torch.cuda.Stream(), torch.cuda.current_stream()
+    x = torch.zeros(8, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        for call in (lambda: dev.pages_copy(pool, src, dst), lambda: dev.pages_free(*state_, 4)):
+            with pytest.raises(TensorLibError, match="captured"):
+                call()
+        x += 1
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(pool, kept) and bool((x == 1).all()) and state_[1].tolist() == [7]
+    g = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(g, stream=side):
+            dev.bind_stream(side)
+            with torch.cuda.stream(main):
+                dev.pages_copy(pool, src, dst)
+    finally:
+        dev.bind_stream(main)
+    for _ in range(3):
+        pool.copy_(kept)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(pool, want)

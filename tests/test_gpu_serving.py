@@ -1132,3 +1132,74 @@ def test_captures_and_another_library_stream(dev):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(pool, want)
+
+
+def test_a_captured_beam_step_with_its_pages(dev):
+    """Selection, histories, fork, copy, extension and release of finished rows in one graph, what works in place included:
+    replayed with other inputs, eager work between the replays, each compared with the eager step and with the plain loops."""
+    requests, beams, page, width, vocab, planes, history = 5, 4, 8, 6, 3000, 3, 60
+    rows = requests * beams
+    n_pages = rows * width + 40
+
+    def inputs(seed):
+        r = np.random.RandomState(seed)
+        tables, lens, refs, _ = state(rows, page, width, seed, 40, r.randint(1, page * width - 1, rows))
+        refs = np.concatenate([refs, np.zeros(n_pages - len(refs), int)])
+        return dict(logits=rand((rows, vocab), seed, 2.5), scores=-torch.rand(rows, generator=torch.Generator().manual_seed(seed)).cuda(), finished=torch.as_tensor(r.rand(rows) < 0.2, device="cuda"),
+                    history=ints(r.randint(0, vocab, (rows, history))), hist_lens=ints(r.randint(1, history, rows)), tables=ints(tables), lens=ints(lens), refs=ints(refs),
+                    pool=rand((planes, n_pages, page, 2, 8), seed + 1))
+
+    def step(s):
+        scores, tokens, parents = dev.beam_select(s["logits"], s["scores"], beams, s["finished"], 2)
+        hist, hist_lens, finished = dev.beam_advance(s["history"], s["hist_lens"], s["finished"], parents, tokens, 2)
+        tables, lens, refs, src, dst, lacking = dev.pages_fork(s["tables"], s["lens"], s["refs"], parents, page)
+        dev.pages_copy(s["pool"], src, dst)
+        short = dev.pages_extend(tables, lens, refs, finished.logical_not().int(), page)
+        forked = tables.clone(), lens.clone(), refs.clone()
+        dev.pages_free(tables, lens, refs, finished, page)
+        return scores, tokens, parents, hist, hist_lens, finished, src, dst, lacking, short, *forked, tables, lens, refs
+
+    side, s = torch.cuda.Stream(), inputs(1)
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(side):
+            dev.bind_stream(side)
+            step(s)
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                out = step(s)
+    finally:
+        dev.bind_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    for seed in (2, 3, 4, 5):
+        fresh = inputs(seed)
+        for name, t in fresh.items():
+            s[name].copy_(t)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = step(fresh)                                         # eager, on inputs of its own
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(s["pool"], fresh["pool"]), seed
+        start = inputs(seed)
+        tables, lens, refs, src, dst = fork_by_hand(*(start[k].cpu().numpy() for k in ("tables", "lens", "refs")), got[2].cpu().tolist(), page)
+        assert got[6].cpu().tolist() == src and got[7].cpu().tolist() == dst and int(got[8]) == int(got[9]) == 0
+        pool = start["pool"]
+        for a, b in zip(src, dst):
+            if a >= 0:
+                pool[:, b] = pool[:, a]
+        assert torch.equal(s["pool"], pool)
+        done = got[5].cpu().tolist()
+        for i in range(rows):
+            if not done[i] and lens[i] % page == 0:
+                tables[i][lens[i] // page] = refs.index(0)
+                refs[refs.index(0)] = 1
+            lens[i] += not done[i]
+        assert [t.cpu().tolist() for t in got[10:13]] == [tables, lens, refs]
+        for i in range(rows):
+            if done[i]:
+                for p in tables[i][: -(-lens[i] // page)]:
+                    refs[p] -= 1
+                tables[i], lens[i] = [-1] * width, 0
+        assert [t.cpu().tolist() for t in got[13:]] == [tables, lens, refs]

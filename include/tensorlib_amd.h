@@ -437,7 +437,8 @@ int tl_rotary_kv_pages_f16(void* q_out, const void* q, size_t q_stride, const vo
  * for every call with these heads, at most n_seqs sequences and a bound of at most max_len; what one call of just these sizes
  * needs is tl_paged_attention_workspace_of_call bytes (0 if none), which may be more for a smaller call.  lens[b] <= 0 gives
  * zeros; lens[b] beyond max_len or the table, or a page out of range among the
- * pages it covers, gives NaN for that sequence.  Scores, weights and sums are fp32, one rounding at the end.
+ * pages it covers, gives NaN for that sequence.  Scores, maxima and sums are fp32, one rounding at the end; in the product with V
+ * a weight is the sum of two halves, off by at most 2^-21 of itself and 2^-35 of the largest.
  * At most 65535 sequences.  out may be q if q is dense. */
 size_t tl_paged_attention_workspace(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len);
 size_t tl_paged_attention_workspace_of_call(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_len);
@@ -477,7 +478,8 @@ int tl_pages_copy(void* pool, size_t plane_stride, size_t page_stride, size_t pa
  * parents_out ([n_batch, n_select], the parent as a row r), best first, equal scores by the lower beam, then the lower
  * token.  finished (bytes, may be NULL): a finished row continues only with end_token, at its own score.  Everything
  * else is at -inf and follows in the same order: other tokens of a finished row, all tokens of a row whose logits
- * hold NaN or +inf or nothing but -inf, or whose score is not finite.  Row sums and comparisons in fp64.
+ * hold NaN or +inf or nothing but -inf, or whose score is not finite.  Scores are compared in fp64; a row's logarithm of the sum, of
+ * fp32 exponentials, is off by at most 2^-20, so continuations of different beams that lie closer may come in either order.
  * n_select <= 64, n_beams <= 1024, at most 65535 rows.  tl_beam_select_workspace bytes are enough for every call with at most as many
  * requests, beams, tokens and continuations. */
 size_t tl_beam_select_workspace(int n_batch, int n_beams, int vocab, int n_select);

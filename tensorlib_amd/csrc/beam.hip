@@ -2,8 +2,10 @@
 //
 // Every beam of a request continues with every token at  score + logit - log sum exp(logits);  the best n of a request
 // go on, equal scores in the order of (beam, token).  A finished beam has one continuation, its end token at its own
-// score.  The sum of a row is held in fp64 and scores are compared in fp64: candidates of different beams may lie
-// closer than an fp32 rounding.
+// score.  Scores are compared in fp64: as fp32 they would be rounded by 2^-20 at a score of -20.  A row's sum takes fp32
+// exponentials and is fp32 within a thread and fp64 from there on.  Its relative error, which is its logarithm's absolute one, is
+// at most 2^-23 for an exponential, 0.8 2^-23 for its argument and eight additions of 2^-24 in turn: below 2^-20.  Continuations
+// of different beams that lie closer may come in either order; within a beam the logits alone decide.
 //
 // Bound by the one pass over the logits (2 bytes each), small requests by latency.  First launch: one workgroup per (row,
 // slice of the vocabulary) holds its slice in registers and leaves the slice's maximum, its sum and its best n

@@ -31,8 +31,9 @@ constexpr int kWaves = 4;
 constexpr int kMinChunk = 128, kMaxChunk = 1024;   // positions of a workgroup, a power of two
 constexpr int kGroupTile = 16;            // query heads that share a pass over K and V
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are kept 2^12 times as large as exp(score - max), in the sum too: as halves they lose nothing down to 2^-36 of
-// the largest one.
+// Weights are kept 2^12 times as large as exp(score - max), in the sum too.  As two halves, the first truncated and the second
+// rounded, a weight is off by at most 2^-21 of itself; where the parts are subnormal or raised to kTiny, by less than 2 kTiny,
+// which is 2^-35 of the largest weight.
 constexpr float kWeightLog2 = 12.f;
 constexpr float kTiny = 5.9604644775390625e-8f;   // 2^-24, the smallest positive half
 
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_kernel(PagedAttnArgs A
                         for (int x = 0; x < VP; ++x) vf[u][r][x] = (vpiece)(half_t)0.f;
                     }
         }
-        // p as the sum of two halves: no bit of it that matters is lost.  hi is rounded towards zero and neither part of a
+        // p as the sum of two halves.  hi is rounded towards zero and neither part of a
         // positive weight becomes zero, so that an infinite value keeps its sign.  The eight (four) positions of a lane
         // come together as A[row = dims, k = position] by exchanges within the lane.
         weights hi, lo;

@@ -60,7 +60,7 @@ struct PageRange {
         end = e < n_pages ? (int)e : n_pages;
         first = load(begin + (int)(threadIdx.x % 64) * 4);
     }
-    // Four counts of the lane; what lies behind the last page counts as 1, taken and not live: f() never sees it.
+    // Four counts of the lane; behind the range's last page zeros, which f() never sees.
     __device__ __forceinline__ int4 load(int p) const {
         int4 r = {0, 0, 0, 0};
         if (p + 4 <= end) __builtin_memcpy(&r, refs + p, 16);

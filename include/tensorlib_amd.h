@@ -479,7 +479,8 @@ int tl_pages_copy(void* pool, size_t plane_stride, size_t page_stride, size_t pa
  * token.  finished (bytes, may be NULL): a finished row continues only with end_token, at its own score.  Everything
  * else is at -inf and follows in the same order: other tokens of a finished row, all tokens of a row whose logits
  * hold NaN or +inf or nothing but -inf, or whose score is not finite.  Scores are compared in fp64; a row's logarithm of the sum, of
- * fp32 exponentials, is off by at most 2^-20, so continuations of different beams that lie closer may come in either order.
+ * fp32 exponentials, is off by at most 2^-20, so continuations of different beams that lie closer may come in either order.  A row
+ * whose logits leave one token (the others at -inf) keeps its score exactly.
  * n_select <= 64, n_beams <= 1024, at most 65535 rows.  tl_beam_select_workspace bytes are enough for every call with at most as many
  * requests, beams, tokens and continuations. */
 size_t tl_beam_select_workspace(int n_batch, int n_beams, int vocab, int n_select);

@@ -5,7 +5,8 @@
 // score.  Scores are compared in fp64: as fp32 they would be rounded by 2^-20 at a score of -20.  A row's sum takes fp32
 // exponentials and is fp32 within a thread and fp64 from there on.  Its relative error, which is its logarithm's absolute one, is
 // at most 2^-23 for an exponential, 0.8 2^-23 for its argument and eight additions of 2^-24 in turn: below 2^-20.  Continuations
-// of different beams that lie closer may come in either order; within a beam the logits alone decide.
+// of different beams that lie closer may come in either order; within a beam the logits alone decide.  (Relative to the largest
+// term, as the pick takes it where that has most of the sum, its own 1.8 2^-23 are added, and what the two share drops out.)
 //
 // Bound by the one pass over the logits (2 bytes each), small requests by latency.  First launch: one workgroup per (row,
 // slice of the vocabulary) holds its slice in registers and leaves the slice's maximum, its sum and its best n
@@ -39,7 +40,7 @@ constexpr int kList = 1024;
 struct SliceStats {
     double sum;                                           // of 2^(logit log2 e - top), NaN if the slice holds NaN or +inf
     float top;                                            // a whole number, kLowest for nothing but -inf
-    float pad;
+    float most;                                           // the largest logit; anything if the sum is NaN or 0
 };
 
 struct BeamArgs {
@@ -157,6 +158,12 @@ __device__ __forceinline__ float from_order(unsigned o) { return __builtin_bit_c
 // t 0.93e-8, which its share of the sum makes 2.5e-8 at most, less than half an fp32 rounding (192 rows of 100003: 23.7 -> 23.3 us).
 constexpr float kLog2e = 1.4426950216293335f, kLog2eRest = 9.253347e-9f;       // the latter d ln 2
 constexpr float kLowest = -131072.f;                      // below every finite half times log2 e
+__device__ __forceinline__ float whole_above(float most) { return fmaxf(ceilf(most * kLog2e), kLowest); }
+__device__ __forceinline__ float power_of(float x, float c) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, -c)); }
+__device__ __forceinline__ float with_rest(float sum, float c) {
+    const float rest = c * kLog2eRest;
+    return __builtin_fmaf(sum, __builtin_fmaf(0.5f * rest, rest, rest), sum);     // e^rest to its square, at most 8.8e-4
+}
 __device__ __forceinline__ int exponent_of(float c, float reference) { return (int)fmaxf(c - reference, -1024.f); }
 
 // NV: 16-byte pieces of logits per thread; a slice is NV * 2048 of them.
@@ -199,15 +206,14 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
         m[0] = __builtin_elementwise_max(__builtin_elementwise_max(m[0], m[1]), __builtin_elementwise_max(m[2], m[3]));
         most[j] = __builtin_elementwise_max(m[0][0], m[0][1]);
         top = __builtin_elementwise_max(top, most[j]);
-        c[j] = fmaxf(ceilf((float)most[j] * kLog2e), kLowest);
+        c[j] = whole_above((float)most[j]);
         c_thread = fmaxf(c_thread, c[j]);
         float p[2] = {0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            p[e % 2] += __builtin_amdgcn_exp2f(__builtin_fmaf((float)v[j][e], kLog2e, -c[j]));
+            p[e % 2] += power_of((float)v[j][e], c[j]);
         }
-        const float rest = c[j] * kLog2eRest, sum = p[0] + p[1];
-        part[j] = __builtin_fmaf(sum, __builtin_fmaf(0.5f * rest, rest, rest), sum);      // e^rest to its square, at most 8.8e-4
+        part[j] = with_rest(p[0] + p[1], c[j]);
     }
     float mine_sum = 0.f;
 #pragma unroll
@@ -233,12 +239,14 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
     unsigned reach = s_bound[0];
 #pragma unroll
     for (int w = 1; w < kBeamWaves; ++w) reach = shared ? min(reach, s_bound[w]) : max(reach, s_bound[w]);
+    SliceStats* stats = A.stats + (size_t)row * A.n_slices + slice;
     if (tid == 0) {
         float c_slice = kLowest;
         double sum = 0.0;
         for (int w = 0; w < kBeamWaves; ++w) c_slice = fmaxf(c_slice, s_c[w]);
         for (int w = 0; w < kBeamWaves; ++w) sum += ldexp(s_sum[w], exponent_of(s_c[w], c_slice));
-        A.stats[(size_t)row * A.n_slices + slice] = {sum, c_slice, 0.f};
+        stats->sum = sum;
+        stats->top = c_slice;
     }
     // what reaches the bound
     const half_t reach_value = (half_t)candidate_logit(reach);
@@ -278,6 +286,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
             if (parts >= 4) rank = join<1>(rank, [](int a, int b) { return a + b; });
             if (parts == 8) rank = join<2>(rank, [](int a, int b) { return a + b; });
             if (tid % parts == 0 && rank < A.n_select) best[rank] = mine;
+            if (tid % parts == 0 && rank == 0) stats->most = candidate_logit(mine);
         }
         for (int i = count + tid; i < A.n_select; i += kBeamThreads) best[i] = 0;       // the slice has no more
         return;
@@ -300,6 +309,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(BeamArgs A) {
 #pragma unroll
         for (int w = 0; w < kBeamWaves; ++w) mine = max(mine, s_best[w]);
         if (tid == 0) best[k] = mine;
+        if (tid == 0 && k == 0) stats->most = candidate_logit(mine);
         below = mine;
     }
 }
@@ -343,10 +353,14 @@ __global__ void __launch_bounds__(THREADS) beam_pick_kernel(BeamArgs A) {
         const bool done = A.finished && A.finished[row0 + b];
         const SliceStats* st = A.stats + (size_t)(row0 + b) * A.n_slices;
         // a finished row has left nothing there, and nothing of what is read for it is used
-        SliceStats mine = lane < A.n_slices ? st[lane] : SliceStats{0.0, -INFINITY, 0.f};
-        float top = mine.top;
-        for (int s = lane + 64; s < A.n_slices; s += 64) top = fmaxf(top, st[s].top);
+        SliceStats mine = lane < A.n_slices ? st[lane] : SliceStats{0.0, -INFINITY, -INFINITY};
+        float top = mine.top, most = mine.most;
+        for (int s = lane + 64; s < A.n_slices; s += 64) {
+            top = fmaxf(top, st[s].top);
+            most = fmaxf(most, st[s].most);
+        }
         top = wave_max(top);
+        most = wave_max(most);
         double sum = 0.0;
         for (int s = lane;;) {
             if (mine.sum != 0.0) sum += mine.sum * exp2((double)mine.top - (double)top);
@@ -355,7 +369,11 @@ __global__ void __launch_bounds__(THREADS) beam_pick_kernel(BeamArgs A) {
             mine = st[s];
         }
         sum = wave_sum(sum);
-        const double base = done ? score : score - ((double)top * 0.69314718055994530942 + log(sum));
+        // Where one token has most of the sum, the logarithm is taken relative to that token's own term, computed as it was in
+        // the sum: the error of its exponential drops out, and a row with one token left continues with probability 1 to the bit.
+        const double own = (double)with_rest(power_of(most, top), top);
+        const double log_sum = sum < 2.0 * own ? (double)most + log(sum / own) : (double)top * 0.69314718055994530942 + log(sum);
+        const double base = done ? score : score - log_sum;
         if (lane == 0) {
             const bool finite = base > -INFINITY && base < INFINITY;
             s_base[b] = finite ? base : -INFINITY;

@@ -1203,3 +1203,22 @@ def test_a_captured_beam_step_with_its_pages(dev):
                     refs[p] -= 1
                 tables[i], lens[i] = [-1] * width, 0
         assert [t.cpu().tolist() for t in got[13:]] == [tables, lens, refs]
+
+
+@pytest.mark.parametrize("batch,beams,vocab,n,masked", [(1, 8, 1, 8, -math.inf), (3, 4, 32000, 4, -math.inf), (2, 8, 100003, 8, -65504.0), (9, 8, 50257, 8, -math.inf), (1, 64, 5000, 64, -math.inf),
+                                                        (1, 3, 600001, 2, -65504.0)])
+def test_beam_select_of_one_allowed_token(dev, batch, beams, vocab, n, masked):
+    """A row with one token left continues with probability 1: its score stays what it was, to the bit, and beams of equal scores
+    come in their order, whatever the token's logit is and wherever it stands."""
+    rows = batch * beams
+    rng = np.random.RandomState(vocab)
+    logits = torch.full((rows, vocab), masked, dtype=torch.float16, device="cuda")
+    token = torch.as_tensor(rng.randint(0, vocab, rows), device="cuda")
+    logits[torch.arange(rows, device="cuda"), token] = rand((rows,), 9, 8.0)
+    for scores in (torch.zeros(rows, device="cuda"), torch.full((rows,), -3.1875, device="cuda"), torch.as_tensor(-rng.randint(0, 3, rows) - 0.3, dtype=torch.float32, device="cuda"),
+                   -20 * torch.rand(rows, generator=torch.Generator().manual_seed(1)).cuda()):
+        got = select_into(dev, logits, scores, None, beams, 0, n)
+        order = torch.sort(scores.view(batch, beams), dim=1, descending=True, stable=True)
+        parents = (order.indices[:, :n] + beams * torch.arange(batch, device="cuda")[:, None]).flatten()
+        assert torch.equal(got[2], parents.int()) and torch.equal(got[1], token[parents].int())
+        assert torch.equal(got[0], scores[parents])

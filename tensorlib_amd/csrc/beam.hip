@@ -19,7 +19,7 @@
 // place in the answer.  A list that overflows (values in an order that defeats the bound) is given up for n rounds of a maximum
 // over the workgroup.
 //
-// 24 requests of 8 beams over 100003 tokens: 13 + 6 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
+// 24 requests of 8 beams over 100003 tokens: 13 + 5.5 us (38 MB: 6 us at the rate of a plain read; the vector pipes are busy
 // for 7 us of the first launch, and its workgroups do not all run at a time).  1 request of 4 beams over 32000: 4 + 4 us,
 // two launches and their memory latencies.  64 beams over 100003, 64 selected: 120 us, most of it the second launch.
 #include <algorithm>
